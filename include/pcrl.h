@@ -34,7 +34,7 @@ extern "C" {
 #define PCRL_MAX_SEG 4
 #define PCRL_MAX_CHANNELS 16
 
-enum { PCRL_DT_F32 = 0, PCRL_DT_U8 = 1, PCRL_DT_BOOL = 2 };
+enum { PCRL_DT_F32 = 0, PCRL_DT_U8 = 1, PCRL_DT_BOOL = 2, PCRL_DT_BF16 = 3, PCRL_DT_F16 = 4 };
 
 /* One observation key ("xyz", "rgb", "pos_encoding", "seg") of the batched
  * observation dict the reference feeds PointCloudBase.preprocess
@@ -597,6 +597,71 @@ int pcrl_gather_scalars_f32(const float* const* src, float* const* dst, const in
  * reads of sac.py:150-159,199-204. */
 int pcrl_gather_scalars_host_f32(const float* const* src, float* const* dst, const int32_t* take_exp, int32_t n,
                                  const pcrl_adam_pending* pending, int32_t n_pending, float* host_out, void* stream);
+
+/* ---- sequence operators: the recurrent core's short causal convolution and selective state space scan, and dropout ----------------------
+ * Activations are PCRL_DT_F32, PCRL_DT_BF16 or PCRL_DT_F16 (one type per call), [B, T, D] with strides in elements for batch and time and
+ * the channels adjacent; parameters, recurrent states of the scan and every sum are float32.  Outputs without strides are dense.
+ *   starts  [B][T] bytes (batch stride starts_sb) or NULL: non-zero where step t is the first of a new sequence -- nothing from before it
+ *           (the incoming state included) reaches it;
+ *   lengths [B] or NULL: batch row b has lengths[b] steps (clamped to 0 ... T).  Outputs and gradients behind them are 0, inputs behind them are
+ *           not looked at, the last state is the one after step lengths[b] - 1 (the incoming one when there is none). */
+typedef struct pcrl_conv_desc {
+    int32_t B, T, D, W;            /* W taps, 1 ... 4 */
+    int32_t dtype, silu;           /* silu != 0: y = pre * sigmoid(pre) */
+    const void* x; int64_t x_sb, x_st;
+    const float* weight;           /* [D][W]; tap W - 1 meets the step itself */
+    const float* bias;             /* [D] or NULL */
+    const void* state;             /* [B][W-1][D] dense, oldest step first, or NULL (zeros) */
+    const uint8_t* starts; int64_t starts_sb;
+    const int32_t* lengths;
+} pcrl_conv_desc;
+/* y [B][T][D], last_state [B][W-1][D] (either may be NULL).  last_state may be the memory of `state` only when T == 1 (the acting step). */
+int pcrl_short_conv_fwd(const pcrl_conv_desc* d, void* y, void* last_state, void* stream);
+int pcrl_short_conv_bwd_workspace_bytes(const pcrl_conv_desc* d, size_t* bytes);
+/* Gradients of sum(y * dy) + sum(last_state * dlast): dx [B][T][D], dweight [D][W], dbias [D] or NULL, dstate [B][W-1][D] or NULL.
+ * dlast may be NULL.  No atomics: the same call gives the same bits. */
+int pcrl_short_conv_bwd(const pcrl_conv_desc* d, const void* dy, int64_t dy_sb, int64_t dy_st, const void* dlast, void* dx, float* dweight,
+                        float* dbias, void* dstate, void* workspace, size_t workspace_bytes, void* stream);
+
+/* h_t = exp(dt_t A) h_{t-1} + dt_t B_t u_t,  y_t = (sum_n C_t h_t + D u_t) * silu(z_t),  dt_t = softplus(dt + dt_bias) (or dt + dt_bias). */
+typedef struct pcrl_ssm_desc {
+    int32_t B, T, D, N;            /* N states per channel, 1 ... 32 */
+    int32_t G, dtype, softplus, _pad;    /* G groups share the channels evenly (D % G == 0); B_t and C_t are per group */
+    const void *u, *dt, *z;        /* z NULL: no gate */
+    int64_t u_sb, u_st, dt_sb, dt_st, z_sb, z_st;
+    const void *Bm, *Cm;           /* [B][T][G][N], states adjacent */
+    int64_t b_sb, b_st, b_sg, c_sb, c_st, c_sg;
+    const float *A, *D_skip, *dt_bias;   /* [D][N]; [D] or NULL; [D] or NULL */
+    const float* state;            /* [B][D][N] dense or NULL (zeros) */
+    const uint8_t* starts; int64_t starts_sb;
+    const int32_t* lengths;
+} pcrl_ssm_desc;
+typedef struct pcrl_ssm_grads {
+    void *du, *ddt, *dz;           /* [B][T][D]; dz only with z */
+    void *dB, *dC;                 /* [B][T][G][N] */
+    float *dA, *dD, *ddt_bias;     /* [D][N]; [D] or NULL; [D] or NULL */
+    float* dstate;                 /* [B][D][N] or NULL */
+} pcrl_ssm_grads;
+/* workspace: what the forward needs (0 for most shapes); saved: what a forward that will be differentiated leaves for its backward (the state
+ * in front of every 16th step); bwd: the backward's workspace. */
+int pcrl_ssm_scan_bytes(const pcrl_ssm_desc* d, size_t* workspace, size_t* saved, size_t* bwd);
+/* y [B][T][D], last_state [B][D][N] (may be NULL); saved NULL: no backward will follow. */
+int pcrl_ssm_scan_fwd(const pcrl_ssm_desc* d, void* y, float* last_state, float* saved, void* workspace, size_t workspace_bytes, void* stream);
+/* Gradients of sum(y * dy) + sum(last_state * dlast) (dlast may be NULL), from the forward's inputs and `saved`.  No atomics: the same call
+ * gives the same bits. */
+int pcrl_ssm_scan_bwd(const pcrl_ssm_desc* d, const float* saved, const void* dy, int64_t dy_sb, int64_t dy_st, const float* dlast,
+                      const pcrl_ssm_grads* g, void* workspace, size_t workspace_bytes, void* stream);
+/* One step (d->T == 1; d->state is read, may not be NULL; lengths are not looked at): y [B][D], state_out [B][D][N] -- the memory of d->state
+ * itself, or memory that does not touch it. */
+int pcrl_ssm_step(const pcrl_ssm_desc* d, void* y, float* state_out, void* stream);
+
+/* out = kept(x) * 65536 / (65536 - threshold) + residual over `rows` x `cols` elements (row strides in elements, columns adjacent; `out`
+ * dense; residual may be NULL), dropped elements are 0 whatever x holds.  Element e = row * cols + col is dropped when half-word e % 8 of
+ * Philox4x32-10(key = seed, counter = (e / 8 lo, e / 8 hi, offset lo, offset hi)) is below threshold (0 ... 65536; half-word 2 w is the low half
+ * of word w); the mask is never stored: the backward is the same call on the gradient.  offset_ptr (device, may be NULL) overrides offset at
+ * run time.  out may be x or residual itself when that one is dense. */
+int pcrl_dropout(const void* x, int64_t x_ld, const void* residual, int64_t residual_ld, void* out, int64_t rows, int64_t cols, int32_t dtype,
+                 int32_t threshold, uint64_t seed, uint64_t offset, const uint64_t* offset_ptr, void* stream);
 
 #ifdef __cplusplus
 }

@@ -11,7 +11,7 @@ LIB_PATH = os.environ.get("PCRL_HIP_LIB") or os.path.join(_HERE, "libpcrl_hip.so
 
 PCRL_MAX_SEG = 4
 PCRL_MAX_CHANNELS = 16
-DT_F32, DT_U8, DT_BOOL = 0, 1, 2
+DT_F32, DT_U8, DT_BOOL, DT_BF16, DT_F16 = 0, 1, 2, 3, 4
 AUG_JITTER, AUG_AFFINE, AUG_SUBSAMPLE, AUG_COLOR = 1, 2, 4, 8
 
 
@@ -91,6 +91,29 @@ class GemmDesc(ctypes.Structure):
                 ("bias_batch_stride", ctypes.c_int64), ("mask_batch_stride", ctypes.c_int64),
                 ("relu", ctypes.c_int32), ("ones_col", ctypes.c_int32), ("accumulate", ctypes.c_int32), ("_pad", ctypes.c_int32),
                 ("C_ones", ctypes.c_void_p), ("c_ones_batch_stride", ctypes.c_int64)]
+
+
+class ConvDesc(ctypes.Structure):
+    _fields_ = [("B", ctypes.c_int32), ("T", ctypes.c_int32), ("D", ctypes.c_int32), ("W", ctypes.c_int32), ("dtype", ctypes.c_int32),
+                ("silu", ctypes.c_int32), ("x", ctypes.c_void_p), ("x_sb", ctypes.c_int64), ("x_st", ctypes.c_int64), ("weight", ctypes.c_void_p),
+                ("bias", ctypes.c_void_p), ("state", ctypes.c_void_p), ("starts", ctypes.c_void_p), ("starts_sb", ctypes.c_int64),
+                ("lengths", ctypes.c_void_p)]
+
+
+class SsmDesc(ctypes.Structure):
+    _fields_ = [("B", ctypes.c_int32), ("T", ctypes.c_int32), ("D", ctypes.c_int32), ("N", ctypes.c_int32), ("G", ctypes.c_int32),
+                ("dtype", ctypes.c_int32), ("softplus", ctypes.c_int32), ("_pad", ctypes.c_int32),
+                ("u", ctypes.c_void_p), ("dt", ctypes.c_void_p), ("z", ctypes.c_void_p),
+                ("u_sb", ctypes.c_int64), ("u_st", ctypes.c_int64), ("dt_sb", ctypes.c_int64), ("dt_st", ctypes.c_int64),
+                ("z_sb", ctypes.c_int64), ("z_st", ctypes.c_int64), ("Bm", ctypes.c_void_p), ("Cm", ctypes.c_void_p),
+                ("b_sb", ctypes.c_int64), ("b_st", ctypes.c_int64), ("b_sg", ctypes.c_int64),
+                ("c_sb", ctypes.c_int64), ("c_st", ctypes.c_int64), ("c_sg", ctypes.c_int64),
+                ("A", ctypes.c_void_p), ("D_skip", ctypes.c_void_p), ("dt_bias", ctypes.c_void_p), ("state", ctypes.c_void_p),
+                ("starts", ctypes.c_void_p), ("starts_sb", ctypes.c_int64), ("lengths", ctypes.c_void_p)]
+
+
+class SsmGrads(ctypes.Structure):
+    _fields_ = [(k, ctypes.c_void_p) for k in ("du", "ddt", "dz", "dB", "dC", "dA", "dD", "ddt_bias", "dstate")]
 
 
 class PcrlError(RuntimeError):
