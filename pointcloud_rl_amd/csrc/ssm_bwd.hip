@@ -13,327 +13,389 @@
 namespace pcrl {
 
 // lo / hi: two values per lane -> one: lanes with the level's bit of their row position clear get lo + partner's lo, the others hi + partner's
-// hi.  Partners: position ^ 7 (half-row mirror; first, because it mixes the low bits), ^ 2, ^ 1, ^ 8: after the four levels every position of the
-// row is in the sum once.  Levels 0 to 3 settle bits 2, 1, 0, 3 of the position.
-template <int LEVEL>
-__device__ __forceinline__ float fold(float lo, float hi, int r) {
-    constexpr int bit = LEVEL == 0 ? 4 : LEVEL == 1 ? 2 : LEVEL == 2 ? 1 : 8;
-    const bool up = (r & bit) != 0;
-    const float keep = up ? hi : lo, send = up ? lo : hi;
-    return keep + dpp_f<LEVEL == 0 ? 0x141 : LEVEL == 1 ? 0x4E : LEVEL == 2 ? 0xB1 : 0x128>(send);
+// hi.  Partners: position ^ 7 (half-row mirror; first, because it mixes the low bits), ^ 8, ^ 2, ^ 1: after the four levels every position of the
+// row is in the sum once.  Levels 0 to 3 settle bits 2, 3, 1, 0 of the position.  The first two -- 12 of the 15 folds of 16 values -- are settled
+// by whole 4-lane banks, so that the second addition writes only its banks and no selection is needed: 2 instructions instead of 3.
+#define PCRL_FOLD_BANKS(R, LO, HI, CTRL, BANKS)                                           \
+    "v_add_f32_dpp %" #R ", %" #LO ", %" #LO " " CTRL " row_mask:0xf bank_mask:0xf\n\t" \
+    "v_add_f32_dpp %" #R ", %" #HI ", %" #HI " " CTRL " row_mask:0xf bank_mask:" BANKS "\n\t"
+template <int LEVEL, int RN>
+__device__ __forceinline__ void fold(float (&out)[RN], const float (&lo)[RN], const float (&hi)[RN], int r) {
+    float o[RN];
+    if constexpr (LEVEL < 2 && RN == 4) {
+        // s_nop 1: the wait states of a DPP read behind the instructions that formed lo and hi
+        if constexpr (LEVEL == 0)
+            asm("s_nop 1\n\t" PCRL_FOLD_BANKS(0, 4, 8, "row_half_mirror", "0xa") PCRL_FOLD_BANKS(1, 5, 9, "row_half_mirror", "0xa")
+                PCRL_FOLD_BANKS(2, 6, 10, "row_half_mirror", "0xa") PCRL_FOLD_BANKS(3, 7, 11, "row_half_mirror", "0xa")
+                : "=&v"(o[0]), "=&v"(o[1]), "=&v"(o[2]), "=&v"(o[3]) : "v"(lo[0]), "v"(lo[1]), "v"(lo[2]), "v"(lo[3]), "v"(hi[0]), "v"(hi[1]), "v"(hi[2]), "v"(hi[3]));
+        else
+            asm("s_nop 1\n\t" PCRL_FOLD_BANKS(0, 4, 8, "row_ror:8", "0xc") PCRL_FOLD_BANKS(1, 5, 9, "row_ror:8", "0xc")
+                PCRL_FOLD_BANKS(2, 6, 10, "row_ror:8", "0xc") PCRL_FOLD_BANKS(3, 7, 11, "row_ror:8", "0xc")
+                : "=&v"(o[0]), "=&v"(o[1]), "=&v"(o[2]), "=&v"(o[3]) : "v"(lo[0]), "v"(lo[1]), "v"(lo[2]), "v"(lo[3]), "v"(hi[0]), "v"(hi[1]), "v"(hi[2]), "v"(hi[3]));
+    } else {
+        constexpr int bit = LEVEL == 0 ? 4 : LEVEL == 1 ? 8 : LEVEL == 2 ? 2 : 1;
+        const bool up = (r & bit) != 0;
+#pragma unroll
+        for (int j = 0; j < RN; ++j) {
+            const float keep = up ? hi[j] : lo[j], send = up ? lo[j] : hi[j];
+            o[j] = keep + dpp_f<LEVEL == 0 ? 0x141 : LEVEL == 1 ? 0x128 : LEVEL == 2 ? 0x4E : 0xB1>(send);
+        }
+    }
+#pragma unroll
+    for (int j = 0; j < RN; ++j) out[j] = o[j];
 }
-// The step whose value a lane at row position r is left with: bits 0 and 2 change places.
-__device__ __forceinline__ int folded_step(int r) { return (r & 10) | ((r & 1) << 2) | ((r >> 2) & 1); }
-// Binary counter of folds: step t = 15 - K arrives; `held` keeps the upper half of each unfinished pair.  After K = 15 each lane holds in
+// The step whose value a lane at row position r is left with.
+__device__ __forceinline__ int folded_step(int r) { return ((r >> 2) & 3) | ((r & 2) << 1) | ((r & 1) << 3); }
+// Binary counter of folds: step t = 15 - K arrives; held[l] keeps the upper half of the unfinished pair of level l.  After K = 15 each lane holds in
 // held[3] its row's sum of the value of step folded_step(r).
-template <int K>
-__device__ __forceinline__ void fold_step(float v, float (&held)[4], int r) {
+template <int K, int RN>
+__device__ __forceinline__ void fold_step(const float (&v)[RN], float (&held)[4][RN], int r) {
     constexpr int t = 15 - K;
-    if constexpr ((t & 1) != 0) { held[0] = v; }
-    else {
-        const float f0 = fold<0>(v, held[0], r);
-        if constexpr ((t & 2) != 0) { held[1] = f0; }
-        else {
-            const float f1 = fold<1>(f0, held[1], r);
-            if constexpr ((t & 4) != 0) { held[2] = f1; }
-            else {
-                const float f2 = fold<2>(f1, held[2], r);
-                held[3] = (t & 8) != 0 ? f2 : fold<3>(f2, held[3], r);
+    if constexpr ((t & 1) != 0) {
+#pragma unroll
+        for (int j = 0; j < RN; ++j) held[0][j] = v[j];
+    } else if constexpr ((t & 2) != 0) {
+        fold<0, RN>(held[1], v, held[0], r);
+    } else {
+        float f[RN];
+        fold<0, RN>(f, v, held[0], r);
+        if constexpr ((t & 4) != 0) {
+            fold<1, RN>(held[2], f, held[1], r);
+        } else {
+            fold<1, RN>(f, f, held[1], r);
+            if constexpr ((t & 8) != 0) {
+                fold<2, RN>(held[3], f, held[2], r);
+            } else {
+                fold<2, RN>(f, f, held[2], r);
+                fold<3, RN>(held[3], f, held[3], r);
             }
         }
     }
 }
-__device__ __forceinline__ float add_swapped32(float a, float b) {       // lower half: a's two halves added, upper half: b's
-    auto x = __builtin_amdgcn_permlane32_swap(f2u(a), f2u(b), false, false);
-    return u2f(x[0]) + u2f(x[1]);
-}
-__device__ __forceinline__ float add_swapped16(float a, float b) {       // even rows: a's row pair added, odd rows: b's
-    auto x = __builtin_amdgcn_permlane16_swap(f2u(a), f2u(b), false, false);
-    return u2f(x[0]) + u2f(x[1]);
-}
 
-template <typename T, int CPW, bool SUMMARY>
-__global__ __launch_bounds__(512) void ssm_bwd_kernel(const SsmParams p) {
-    constexpr int NS = CPW / 16, V = CPW / 16, ROWS = 64 / CPW;
+// LDS per wave, in floats: the three [channel][step] tiles, softplus slopes of the loading layout, three [state row][step][channel] partial sums.
+template <bool SUMMARY> constexpr int ssm_bwd_wave_lds() { return SUMMARY ? 2 * kInTile : 3 * kInTile + 256 + 3 * kPartTile; }
+
+template <typename T, int RN, int NG, bool VEC, bool SUMMARY>
+__global__ __launch_bounds__(256, 2) void ssm_bwd_kernel(const SsmParams p) {
+    constexpr int kWave = ssm_bwd_wave_lds<SUMMARY>();
     extern __shared__ float lds[];
-    const int groups = p.S * ROWS;                      // partial sums over the states of one (step, channel)
-    float* s_dt = lds;                                  // [16][CPW]
-    float* s_du = s_dt + kTile * CPW;
-    float* s_ds = s_du + kTile * CPW;
-    float* s_gb = s_ds + kTile * CPW;                   // [groups][16][CPW]: sum_n g B
-    float* s_aw = s_gb + groups * kTile * CPW;          // ... sum_n A w
-    float* s_y = s_aw + groups * kTile * CPW;           // ... sum_n C h (only with a gate)
-    const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, r = lane & 15;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+    float* s_dt = lds + wave * kWave;                   // [channel][step]
+    float* s_ds = s_dt + kInTile;
+    float* s_du = s_ds + kInTile;
+    float* s_slope = s_du + kInTile;
+    float* s_gb = s_slope + 256;                        // [state row][step][channel]: sum_n g B
+    float* s_aw = s_gb + kPartTile;                     // ... sum_n A w
+    float* s_y = s_aw + kPartTile;                      // ... sum_n C h
+    float* s_bc = lds + 4 * kWave;                      // [4 waves][dB, dC][16 steps][states]: the four waves' sums over their channels
     int blk, chunk, b0;
     ssm_where(p, blk, chunk, b0);
     if (SUMMARY && chunk == 0) return;                  // nobody ends at the first chunk's summary
-    const int g = blk / p.nblk, c_first = (blk - g * p.nblk) * CPW;
+    const int g = blk / p.nblk, c_first = (blk - g * p.nblk) * 64 + wave * 16;
+    const int left = p.Dg - c_first;                    // channels from this wave's first on; <= 0: it only takes part in the barriers
+    if (SUMMARY && left <= 0) return;
+    const int d_first = left > 0 ? g * p.Dg + c_first : 0;
     const int tile0 = chunk * p.chunk_tiles, tile1 = tile0 + p.chunk_tiles < p.ntile ? tile0 + p.chunk_tiles : p.ntile;
 
-    const bool item = tid < 256;
-    const int row = (tid & 255) / 16, c0 = ((tid & 255) % 16) * V;
-    const int left = p.Dg - c_first - c0, nv = item ? (left < V ? left : V) : 0;
-    const int d0 = g * p.Dg + c_first + c0;
-    float bias[V], skip[V], d_skip[V], d_bias[V];
+    const int row = lane >> 2, c0 = (lane & 3) * 4, nv = left - c0 < 4 ? left - c0 : 4;
+    unsigned cc[4];
+    float d_skip[4], d_bias[4];
 #pragma unroll
-    for (int i = 0; i < V; ++i) {
-        bias[i] = i < nv && p.dt_bias ? p.dt_bias[d0 + i] : 0.0f;
-        skip[i] = i < nv && p.Dskip ? p.Dskip[d0 + i] : 0.0f;
+    for (int i = 0; i < 4; ++i) {
+        cc[i] = c0 + i < left ? c0 + i : (VEC || left <= 0 ? 0 : left - 1);
         d_skip[i] = d_bias[i] = 0.0f;
     }
-    const int ch = lane % CPW, n0 = wave * 4 + (lane / CPW) * NS;
-    const int dch = g * p.Dg + c_first + ch;
-    const bool has = c_first + ch < p.Dg, walks = wave < p.S;
-    float A[NS], A2[NS], dA[NS];
+    const int ch = lane & 15, q = lane >> 4, dch = d_first + ch;
+    const bool has = ch < left;
+    auto n0 = [&](int k) { return (k * 4 + q) * RN; };
+    auto count = [&](int k) { const int n = p.N - n0(k); return has ? (n < RN ? n : RN) : 0; };
+    unsigned nn[NG][RN];
+    float A2[NG][RN], dA[NG][RN];
 #pragma unroll
-    for (int j = 0; j < NS; ++j) {
-        A[j] = walks && has && n0 + j < p.N ? p.A[(long long)dch * p.N + n0 + j] : 0.0f;
-        A2[j] = A[j] * kLog2e;
-        dA[j] = 0.0f;
+    for (int k = 0; k < NG; ++k) {
+        const RawVec<float, RN> a = raw_load<float, RN>(p.A + (long long)dch * p.N + n0(k), count(k), p.vec_n);
+#pragma unroll
+        for (int j = 0; j < RN; ++j) {
+            A2[k][j] = a.v[j] * kLog2e;
+            dA[k][j] = 0.0f;
+            nn[k][j] = n0(k) + j < p.N ? n0(k) + j : (VEC ? 0 : p.N - 1);
+        }
     }
+    const bool clean = left >= 16 && p.N == 4 * RN * NG;
+    const unsigned o_h = (has ? ch : 0) * (unsigned)p.N;
 
     for (int b = b0; b < p.B; b += p.b_step) {
         const int len = ssm_length(p, b);
-        const T* pu = (const T*)p.u + b * p.u_sb + d0;
-        const T* pd = (const T*)p.dt + b * p.dt_sb + d0;
-        const T* pz = p.z ? (const T*)p.z + b * p.z_sb + d0 : nullptr;
-        const T* pg = (const T*)p.dy + b * p.dy_sb + d0;
+        const T* pu = (const T*)p.u + b * p.u_sb + d_first;
+        const T* pd = (const T*)p.dt + b * p.dt_sb + d_first;
+        const T* pz = p.z ? (const T*)p.z + b * p.z_sb + d_first : nullptr;
+        const T* pg = (const T*)p.dy + b * p.dy_sb + d_first;
         const T* pB = (const T*)p.Bm + b * p.b_sb + g * p.b_sg;
         const T* pC = (const T*)p.Cm + b * p.c_sb + g * p.c_sg;
         const uint8_t* ps = p.starts ? p.starts + b * p.starts_sb : nullptr;
-        const long long orow = (long long)b * p.T;      // dense outputs
-        float gc[NS];                                   // what the steps behind add to g of this one
+        const long long obase = (long long)b * p.T * p.D + d_first;           // dense outputs
+        float gc[NG][RN];                               // what the steps behind add to g of this one
 #pragma unroll
-        for (int j = 0; j < NS; ++j)
-            gc[j] = !SUMMARY && walks && has && n0 + j < p.N && p.dlast ? p.dlast[((long long)b * p.D + dch) * p.N + n0 + j] : 0.0f;
-        if (!SUMMARY && walks && has) {
-            for (int c = p.nchunk - 1; c > chunk; --c)
+        for (int k = 0; k < NG; ++k) {
+            const RawVec<float, RN> l = raw_load<float, RN>(p.dlast + ((long long)b * p.D + dch) * p.N + n0(k), !SUMMARY && p.dlast ? count(k) : 0, p.vec_n);
 #pragma unroll
-                for (int j = 0; j < NS; ++j)
-                    if (n0 + j < p.N) {
-                        const long long at = (((long long)b * p.nchunk + c) * p.N + n0 + j) * p.D + dch;
-                        const float P = p.sum_p[at], s = p.sum_s[at];
-                        gc[j] = P == 0.0f ? s : __builtin_fmaf(P, gc[j], s);
-                    }
+            for (int j = 0; j < RN; ++j) gc[k][j] = l.v[j];
+            if (!SUMMARY) {
+                for (int c = p.nchunk - 1; c > chunk; --c) {
+                    const long long at = (((long long)b * p.nchunk + c) * p.D + dch) * p.N + n0(k);
+                    const RawVec<float, RN> P = raw_load<float, RN>(p.sum_p + at, count(k), p.vec_n), S = raw_load<float, RN>(p.sum_s + at, count(k), p.vec_n);
+#pragma unroll
+                    for (int j = 0; j < RN; ++j) gc[k][j] = P.v[j] == 0.0f ? S.v[j] : __builtin_fmaf(P.v[j], gc[k][j], S.v[j]);
+                }
+            }
         }
         float dt_sum = 0.0f;
         bool cut = false;
 
-        RawVec<T, V> nu, nd, nz, ng;
-        T nB[NS], nC[NS];
-        float nh[NS];
-        unsigned char nst;
-        auto fetch = [&](int tile) {
-            const int t = tile * kTile + row, n = t < len ? nv : 0;
-            if (!SUMMARY) nu = raw_load<T, V>(pu + t * p.u_st, n, p.vec);
-            nd = raw_load<T, V>(pd + t * p.dt_st, n, p.vec);
-            if (pz) nz = raw_load<T, V>(pz + t * p.z_st, n, p.vec);
-            ng = raw_load<T, V>(pg + t * p.dy_st, n, p.vec);
-            const int tl = tile * kTile + r;
-            const bool on = walks && tl < len;
+        RawVec<T, 4> nu, nd, nz, ng;
+        RawVec<T, RN> nB[NG], nC[NG];
+        RawVec<float, RN> nh[NG];
+        unsigned nst = 0;
+        auto fetch = [&](int tile) {                    // rows behind the length read the last one
+            const long long t0 = (long long)tile * kTile;
+            const int last = len - 1 - (int)t0, r = row < last ? row : last, rn = ch < last ? ch : last;
+            if (!SUMMARY) nu = lane_load<T, 4, VEC>(pu + t0 * p.u_st, r * (unsigned)p.u_st, cc);
+            nd = lane_load<T, 4, VEC>(pd + t0 * p.dt_st, r * (unsigned)p.dt_st, cc);
+            if (pz) nz = lane_load<T, 4, VEC>(pz + t0 * p.z_st, r * (unsigned)p.z_st, cc);
+            ng = lane_load<T, 4, VEC>(pg + t0 * p.dy_st, r * (unsigned)p.dy_st, cc);
 #pragma unroll
-            for (int j = 0; j < NS; ++j) {
-                if (!SUMMARY) nB[j] = on && n0 + j < p.N ? pB[tl * p.b_st + n0 + j] : (T)0.0f;
-                nC[j] = on && n0 + j < p.N ? pC[tl * p.c_st + n0 + j] : (T)0.0f;
-                if (!SUMMARY) nh[j] = walks && has && n0 + j < p.N ? p.saved[(((long long)b * p.ntile + tile) * p.N + n0 + j) * p.D + dch] : 0.0f;
+            for (int k = 0; k < NG; ++k) {
+                if (!SUMMARY) nB[k] = lane_load<T, RN, VEC>(pB + t0 * p.b_st, rn * (unsigned)p.b_st, nn[k]);
+                nC[k] = lane_load<T, RN, VEC>(pC + t0 * p.c_st, rn * (unsigned)p.c_st, nn[k]);
+                if (!SUMMARY) nh[k] = lane_load<float, RN, VEC>(p.saved + (((long long)b * p.ntile + tile) * p.D + d_first) * p.N, o_h, nn[k]);
             }
-            nst = ps && tl < len ? ps[tl] : (unsigned char)0;
+            if (ps) nst = ch <= last ? ps[t0 + rn] : 0;
         };
         const int live = (len + kTile - 1) / kTile, end = tile1 < live ? tile1 : live;
         if (!SUMMARY) {                                 // steps behind the length: zeros
-            float none[V];
-#pragma unroll
-            for (int i = 0; i < V; ++i) none[i] = 0.0f;
+            const float none[4] = {0.0f, 0.0f, 0.0f, 0.0f};
             for (int tile = tile0 > live ? tile0 : live; tile < tile1; ++tile) {
-                const int t = tile * kTile + row, n = t < p.T ? nv : 0;
-                raw_store<T, V>((T*)p.du + (orow + t) * p.D + d0, none, n, p.vec);
-                raw_store<T, V>((T*)p.ddt + (orow + t) * p.D + d0, none, n, p.vec);
-                if (pz) raw_store<T, V>((T*)p.dz + (orow + t) * p.D + d0, none, n, p.vec);
+                const long long at = obase + (long long)tile * kTile * p.D;
+                const int n = tile * kTile + row < p.T ? nv : 0;
+                const unsigned o = row * (unsigned)p.D + c0;
+                lane_store<T, 4, VEC>((T*)p.du + at, o, none, n);
+                lane_store<T, 4, VEC>((T*)p.ddt + at, o, none, n);
+                if (pz) lane_store<T, 4, VEC>((T*)p.dz + at, o, none, n);
             }
         }
         if (tile0 < end) fetch(end - 1);
         for (int tile = end - 1; tile >= tile0; --tile) {
             const int t0 = tile * kTile;
-            const bool here = t0 + row < len;
-            float u[V], z[V], gy[V], dt[V], slope[V], ds[V], sig[V], Bv[NS], Cv[NS], h0[NS];
+            const bool plain = clean && t0 + kTile <= len, here = t0 + row < len;
+            RawVec<T, 4> ru = nu, rz = nz, rg = ng;     // kept as they came: half the registers of a 16-bit type
+            float Bv[NG][RN], Cv[NG][RN], h0[NG][RN];
 #pragma unroll
-            for (int i = 0; i < V; ++i) {
-                u[i] = !SUMMARY ? (float)nu.v[i] : 0.0f;
-                z[i] = pz ? (float)nz.v[i] : 0.0f;
-                gy[i] = (float)ng.v[i];
-                const float raw = (float)nd.v[i] + bias[i];
-                slope[i] = 1.0f;
-                dt[i] = p.softplus ? softplus_(raw, slope[i]) : raw;
-                dt[i] = here ? dt[i] : 0.0f;
-                sig[i] = pz ? sigmoidf_(z[i]) : 0.0f;
-                ds[i] = pz ? gy[i] * (z[i] * sig[i]) : gy[i];
+            for (int k = 0; k < NG; ++k)
+#pragma unroll
+                for (int j = 0; j < RN; ++j) {
+                    Bv[k][j] = !SUMMARY ? (float)nB[k].v[j] : 0.0f;
+                    Cv[k][j] = (float)nC[k].v[j];
+                    h0[k][j] = !SUMMARY ? nh[k].v[j] : 0.0f;
+                }
+            if (!plain) {                               // what does not exist counts for nothing (also in the sums over the channels)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const bool on = here && i < nv;
+                    ru.v[i] = on && !SUMMARY ? ru.v[i] : (T)0.0f;
+                    rz.v[i] = on && pz ? rz.v[i] : (T)0.0f;
+                    rg.v[i] = on ? rg.v[i] : (T)0.0f;
+                }
+#pragma unroll
+                for (int k = 0; k < NG; ++k)
+#pragma unroll
+                    for (int j = 0; j < RN; ++j) {
+                        const bool on = t0 + ch < len && n0(k) + j < p.N;
+                        Bv[k][j] = on ? Bv[k][j] : 0.0f;
+                        Cv[k][j] = on ? Cv[k][j] : 0.0f;
+                        h0[k][j] = j < count(k) ? h0[k][j] : 0.0f;
+                    }
             }
-            if (item) {
 #pragma unroll
-                for (int i = 0; i < V; ++i) {
-                    s_dt[row * CPW + c0 + i] = dt[i];
-                    if (!SUMMARY) s_du[row * CPW + c0 + i] = dt[i] * u[i];
-                    s_ds[row * CPW + c0 + i] = ds[i];
+            for (int i = 0; i < 4; ++i) {
+                const float raw = (float)nd.v[i] + (i < nv && p.dt_bias ? p.dt_bias[d_first + c0 + i] : 0.0f), gy = (float)rg.v[i];
+                float slope = 1.0f, dt = p.softplus ? softplus_(raw, slope) : raw;
+                if (!plain) dt = here && i < nv ? dt : 0.0f;
+                s_dt[(c0 + i) * kInLd + row] = dt;
+                const float z = pz ? (float)rz.v[i] : 0.0f;
+                s_ds[(c0 + i) * kInLd + row] = pz ? gy * (z * sigmoidf_(z)) : gy;
+                if (!SUMMARY) {
+                    s_du[(c0 + i) * kInLd + row] = dt * (float)ru.v[i];
+                    s_slope[i * 64 + lane] = slope;
                 }
             }
-#pragma unroll
-            for (int j = 0; j < NS; ++j) {
-                Bv[j] = !SUMMARY ? (float)nB[j] : 0.0f;
-                Cv[j] = (float)nC[j];
-                h0[j] = !SUMMARY ? nh[j] : 0.0f;
-            }
-            const unsigned starts = ssm_start_bits(nst);
+            const unsigned starts = ps ? ssm_start_bits(nst) : 0u;
+            if constexpr (SUMMARY) wave_lds_fence();
+            else __syncthreads();                       // the last tile's s_bc has been read
             if (tile > tile0) fetch(tile - 1);
-            __syncthreads();
-            if (walks) {
-                const int at = (wave * ROWS + lane / CPW) * (kTile * CPW) + ch;
-                auto walk = [&](auto with_starts) {
-                    constexpr bool WS = decltype(with_starts)::value;
-                    if constexpr (SUMMARY) {
-                        static_for<kTile>([&](auto ki) {
-                            constexpr int t = 15 - decltype(ki)::value;
-                            const float dt_ = s_dt[t * CPW + ch], ds_ = s_ds[t * CPW + ch];
+            auto walk = [&](auto with_starts) {
+                constexpr bool WS = decltype(with_starts)::value;
+                if constexpr (SUMMARY) {
+                    static_for<4>([&](auto gi) {
+                        constexpr int tg = 12 - decltype(gi)::value * 4;
+                        const f32x4 dt4 = *(const f32x4*)(s_dt + ch * kInLd + tg), ds4 = *(const f32x4*)(s_ds + ch * kInLd + tg);
+                        static_for<4>([&](auto ti) {
+                            constexpr int i = 3 - decltype(ti)::value, t = tg + i;
                             const bool fresh = WS && ((starts >> t) & 1u);
 #pragma unroll
-                            for (int j = 0; j < NS; ++j) {
-                                const float gt = __builtin_fmaf(row_bcast<t>(Cv[j]), ds_, gc[j]);
-                                const float next = gt * __builtin_amdgcn_exp2f(dt_ * A2[j]);
-                                gc[j] = fresh ? 0.0f : next;
-                            }
-                            dt_sum += dt_;
-                        });
-                    } else {
-                        float a[kTile][NS], h[kTile][NS];
-                        static_for<kTile>([&](auto ti) {
-                            constexpr int t = decltype(ti)::value;
-                            const float dt_ = s_dt[t * CPW + ch], du_ = s_du[t * CPW + ch];
-                            const bool fresh = WS && ((starts >> t) & 1u);
-                            float acc = 0.0f;
+                            for (int k = 0; k < NG; ++k) {
+                                fma_row_bcast<t, RN>(gc[k], Cv[k], ds4[i]);
 #pragma unroll
-                            for (int j = 0; j < NS; ++j) {
-                                const float x = du_ * row_bcast<t>(Bv[j]), e = __builtin_amdgcn_exp2f(dt_ * A2[j]);
-                                const float hn = __builtin_fmaf(e, t == 0 ? h0[j] : h[t == 0 ? 0 : t - 1][j], x);
-                                a[t][j] = fresh ? 0.0f : e;
-                                h[t][j] = fresh ? x : hn;
-                                acc = j == 0 ? h[t][j] * row_bcast<t>(Cv[j]) : __builtin_fmaf(row_bcast<t>(Cv[j]), h[t][j], acc);
+                                for (int j = 0; j < RN; ++j) {
+                                    const float next = gc[k][j] * __builtin_amdgcn_exp2f(dt4[i] * A2[k][j]);
+                                    gc[k][j] = fresh ? 0.0f : next;
+                                }
                             }
-                            if (p.z) s_y[at + t * CPW] = acc;
+                            dt_sum += dt4[i];
                         });
-                        float hb[NS][4], hc[NS][4];
-                        static_for<kTile>([&](auto ki) {
-                            constexpr int K = decltype(ki)::value, t = 15 - K;
-                            const float dt_ = s_dt[t * CPW + ch], du_ = s_du[t * CPW + ch], ds_ = s_ds[t * CPW + ch];
-                            const bool fresh = WS && ((starts >> t) & 1u);
-                            float gb = 0.0f, aw = 0.0f;
+                    });
+                } else {
+                    static_for<NG>([&](auto kc) {
+                        constexpr int k = decltype(kc)::value;
+                        float a[kTile][RN], h[kTile][RN];
+                        static_for<4>([&](auto gi) {
+                            constexpr int tg = decltype(gi)::value * 4;
+                            __builtin_amdgcn_sched_barrier(0);       // four steps at a time: interleaving all sixteen spills
+                            const f32x4 dt4 = *(const f32x4*)(s_dt + ch * kInLd + tg), du4 = *(const f32x4*)(s_du + ch * kInLd + tg);
+                            static_for<4>([&](auto ti) {
+                                constexpr int i = decltype(ti)::value, t = tg + i;
+                                const bool fresh = WS && ((starts >> t) & 1u);
+                                float acc = 0.0f;
 #pragma unroll
-                            for (int j = 0; j < NS; ++j) {
-                                const float gt = __builtin_fmaf(row_bcast<t>(Cv[j]), ds_, gc[j]);
-                                gb = j == 0 ? gt * row_bcast<t>(Bv[j]) : __builtin_fmaf(row_bcast<t>(Bv[j]), gt, gb);
-                                const float gd = gt * a[t][j];
-                                float w = gd * (t == 0 ? h0[j] : h[t == 0 ? 0 : t - 1][j]);
-                                if (WS) w = fresh ? 0.0f : w;
-                                aw = j == 0 ? w * A[j] : __builtin_fmaf(w, A[j], aw);
-                                dA[j] = __builtin_fmaf(w, dt_, dA[j]);
-                                gc[j] = gd;
-                                fold_step<K>(gt * du_, hb[j], r);
-                                fold_step<K>(ds_ * h[t][j], hc[j], r);
-                            }
-                            s_gb[at + t * CPW] = gb;
-                            s_aw[at + t * CPW] = aw;
+                                for (int j = 0; j < RN; ++j) {
+                                    const float x = du4[i] * row_bcast<t>(Bv[k][j]), e = __builtin_amdgcn_exp2f(dt4[i] * A2[k][j]);
+                                    const float hn = __builtin_fmaf(e, t == 0 ? h0[k][j] : h[t == 0 ? 0 : t - 1][j], x);
+                                    a[t][j] = fresh ? 0.0f : e;
+                                    h[t][j] = fresh ? x : hn;
+                                }
+                                dot_row_bcast<t, RN>(acc, Cv[k], h[t]);
+                                s_y[q * kPartLd + t * 16 + ch] = k == 0 ? acc : acc + s_y[q * kPartLd + t * 16 + ch];
+                            });
                         });
-                        // a lane of a row: one step.  CPW = 64: the four rows hold parts of the sums of 4 states -> one state per row;
-                        // CPW = 32: two row pairs with 2 states each -> likewise; CPW = 16: a row is a state already.
-                        float vb, vc;
-                        if constexpr (CPW == 64) {
-                            vb = add_swapped16(add_swapped32(hb[0][3], hb[2][3]), add_swapped32(hb[1][3], hb[3][3]));
-                            vc = add_swapped16(add_swapped32(hc[0][3], hc[2][3]), add_swapped32(hc[1][3], hc[3][3]));
-                        } else if constexpr (CPW == 32) {
-                            vb = add_swapped16(hb[0][3], hb[1][3]);
-                            vc = add_swapped16(hc[0][3], hc[1][3]);
-                        } else {
-                            vb = hb[0][3], vc = hc[0][3];
-                        }
-                        const int n = wave * 4 + (lane >> 4), ts = t0 + folded_step(r);
-                        if (n < p.N && ts < len) {
-                            const long long o = (((long long)blk * p.B + b) * p.T + ts) * p.N + n;
-                            p.part_b[o] = vb;
-                            p.part_c[o] = vc;
-                        }
+                        float hb[4][RN], hc[4][RN];
+                        static_for<4>([&](auto gi) {
+                            constexpr int tg = 12 - decltype(gi)::value * 4;
+                            __builtin_amdgcn_sched_barrier(0);
+                            const f32x4 dt4 = *(const f32x4*)(s_dt + ch * kInLd + tg), du4 = *(const f32x4*)(s_du + ch * kInLd + tg),
+                                        ds4 = *(const f32x4*)(s_ds + ch * kInLd + tg);
+                            static_for<4>([&](auto ti) {
+                                constexpr int i = 3 - decltype(ti)::value, t = tg + i;
+                                const bool fresh = WS && ((starts >> t) & 1u);
+                                float gb = 0.0f, aw = 0.0f, vb[RN], vc[RN];
+                                fma_row_bcast<t, RN>(gc[k], Cv[k], ds4[i]);          // g_t
+                                dot_row_bcast<t, RN>(gb, Bv[k], gc[k]);
+#pragma unroll
+                                for (int j = 0; j < RN; ++j) {
+                                    vb[j] = gc[k][j] * du4[i];
+                                    vc[j] = ds4[i] * h[t][j];
+                                    const float gd = gc[k][j] * a[t][j];
+                                    float w = gd * (t == 0 ? h0[k][j] : h[t == 0 ? 0 : t - 1][j]);
+                                    if (WS) w = fresh ? 0.0f : w;
+                                    aw = j == 0 ? w * A2[k][j] : __builtin_fmaf(w, A2[k][j], aw);
+                                    dA[k][j] = __builtin_fmaf(w, dt4[i], dA[k][j]);
+                                    gc[k][j] = gd;
+                                }
+                                fold_step<15 - t, RN>(vb, hb, ch);
+                                fold_step<15 - t, RN>(vc, hc, ch);
+                                const int at = q * kPartLd + t * 16 + ch;
+                                s_gb[at] = k == 0 ? gb : gb + s_gb[at];
+                                s_aw[at] = k == 0 ? aw : aw + s_aw[at];
+                            });
+                        });
+                        // this wave's sums over its channels, [step][state]: lane (q, ch) has step folded_step(ch), states n0(k) ...
+                        float* out = s_bc + wave * (2 * 16 * 4 * RN * NG) + folded_step(ch) * (4 * RN * NG) + n0(k);
+#pragma unroll
+                        for (int j = 0; j < RN; ++j) { out[j] = hb[3][j]; out[16 * 4 * RN * NG + j] = hc[3][j]; }
+                    });
+                }
+            };
+            if (starts) { walk(std::true_type{}); cut = true; }
+            else walk(std::false_type{});
+            wave_lds_fence();
+            if constexpr (!SUMMARY) {
+                f32x4 gb = *(const f32x4*)(s_gb + row * 16 + c0), aw = *(const f32x4*)(s_aw + row * 16 + c0), ys = *(const f32x4*)(s_y + row * 16 + c0);
+#pragma unroll
+                for (int k = 1; k < 4; ++k) {
+                    gb += *(const f32x4*)(s_gb + k * kPartLd + row * 16 + c0);
+                    aw += *(const f32x4*)(s_aw + k * kPartLd + row * 16 + c0);
+                    ys += *(const f32x4*)(s_y + k * kPartLd + row * 16 + c0);
+                }
+                float o_u[4], o_dt[4], o_z[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const float u = (float)ru.v[i], z = pz ? (float)rz.v[i] : 0.0f, gy = (float)rg.v[i], dt = s_dt[(c0 + i) * kInLd + row];
+                    const float sig = pz ? sigmoidf_(z) : 0.0f, ds = pz ? gy * (z * sig) : gy;
+                    const float skip = i < nv && p.Dskip ? p.Dskip[d_first + c0 + i] : 0.0f;
+                    o_u[i] = __builtin_fmaf(dt, gb[i], skip * ds);
+                    o_dt[i] = __builtin_fmaf(aw[i], kLn2, u * gb[i]) * s_slope[i * 64 + lane];         // the walk summed A log2(e) w
+                    if (!plain) {
+                        o_u[i] = here ? o_u[i] : 0.0f;
+                        o_dt[i] = here ? o_dt[i] : 0.0f;
                     }
-                };
-                if (starts) { walk(std::true_type{}); cut = true; }
-                else walk(std::false_type{});
-            }
-            __syncthreads();
-            if (!SUMMARY && item) {
-                float gb[V], aw[V], ys[V], o_u[V], o_dt[V], o_z[V];
-#pragma unroll
-                for (int i = 0; i < V; ++i) gb[i] = aw[i] = ys[i] = 0.0f;
-                for (int s = 0; s < groups; ++s)
-#pragma unroll
-                    for (int i = 0; i < V; ++i) {
-                        const int at = s * (kTile * CPW) + row * CPW + c0 + i;
-                        gb[i] += s_gb[at];
-                        aw[i] += s_aw[at];
-                        if (pz) ys[i] += s_y[at];
-                    }
-#pragma unroll
-                for (int i = 0; i < V; ++i) {
-                    o_u[i] = __builtin_fmaf(dt[i], gb[i], skip[i] * ds[i]);
-                    o_dt[i] = here ? __builtin_fmaf(u[i], gb[i], aw[i]) * slope[i] : 0.0f;
-                    if (!here) o_u[i] = 0.0f;
-                    const float y = __builtin_fmaf(skip[i], u[i], ys[i]);
-                    o_z[i] = gy[i] * y * (sig[i] + z[i] * sig[i] * (1.0f - sig[i]));
-                    d_skip[i] = __builtin_fmaf(ds[i], u[i], d_skip[i]);
+                    o_z[i] = gy * __builtin_fmaf(skip, u, ys[i]) * (sig + z * sig * (1.0f - sig));
+                    if (!plain) o_z[i] = here ? o_z[i] : 0.0f;
+                    d_skip[i] = __builtin_fmaf(ds, u, d_skip[i]);
                     d_bias[i] += o_dt[i];
                 }
+                const long long to = obase + (long long)t0 * p.D;
+                const unsigned o = row * (unsigned)p.D + c0;
                 const int n = t0 + row < p.T ? nv : 0;
-                raw_store<T, V>((T*)p.du + (orow + t0 + row) * p.D + d0, o_u, n, p.vec);
-                raw_store<T, V>((T*)p.ddt + (orow + t0 + row) * p.D + d0, o_dt, n, p.vec);
-                if (pz) raw_store<T, V>((T*)p.dz + (orow + t0 + row) * p.D + d0, o_z, n, p.vec);
+                lane_store<T, 4, VEC>((T*)p.du + to, o, o_u, n);
+                lane_store<T, 4, VEC>((T*)p.ddt + to, o, o_dt, n);
+                if (pz) lane_store<T, 4, VEC>((T*)p.dz + to, o, o_z, n);
+                // dB and dC of the tile over the workgroup's 64 channels
+                __syncthreads();
+                constexpr int W = 4 * RN * NG;          // states as they stand in LDS (N of them exist)
+                for (int e = threadIdx.x; e < 2 * 16 * W; e += 256) {
+                    const float* src = s_bc + e;
+                    const float v = (src[0] + src[2 * 16 * W]) + (src[2 * 2 * 16 * W] + src[3 * 2 * 16 * W]);
+                    const int which = e / (16 * W), t = (e / W) % 16, n_ = e % W;
+                    if (n_ < p.N && t0 + t < len) (which ? p.part_c : p.part_b)[(((long long)blk * p.B + b) * p.T + t0 + t) * p.N + n_] = v;
+                }
             }
         }
-        if (walks && has) {
 #pragma unroll
-            for (int j = 0; j < NS; ++j)
-                if (n0 + j < p.N) {
-                    if (SUMMARY) {
-                        const long long at = (((long long)b * p.nchunk + chunk) * p.N + n0 + j) * p.D + dch;
-                        p.sum_p[at] = cut ? 0.0f : __builtin_amdgcn_exp2f(dt_sum * A2[j]);
-                        p.sum_s[at] = gc[j];
-                    } else if (chunk == 0 && p.dstate) {
-                        p.dstate[((long long)b * p.D + dch) * p.N + n0 + j] = gc[j];
-                    }
-                }
+        for (int k = 0; k < NG; ++k) {
+            if (SUMMARY) {
+                const long long at = (((long long)b * p.nchunk + chunk) * p.D + dch) * p.N + n0(k);
+                float P[RN];
+#pragma unroll
+                for (int j = 0; j < RN; ++j) P[j] = cut ? 0.0f : __builtin_amdgcn_exp2f(dt_sum * A2[k][j]);
+                raw_store<float, RN>(p.sum_p + at, P, count(k), p.vec_n);
+                raw_store<float, RN>(p.sum_s + at, gc[k], count(k), p.vec_n);
+            } else if (chunk == 0 && p.dstate) {
+                raw_store<float, RN>(p.dstate + ((long long)b * p.D + dch) * p.N + n0(k), gc[k], count(k), p.vec_n);
+            }
         }
     }
-    if (SUMMARY) return;
-    // this workgroup's part of dA, dD, ddt_bias
-    const long long part = (long long)b0 * p.nchunk + chunk;
-    if (walks && has) {
+    if constexpr (!SUMMARY) {
+        // this wave's part of dA, dD, ddt_bias
+        const long long part = (long long)b0 * p.nchunk + chunk;
 #pragma unroll
-        for (int j = 0; j < NS; ++j)
-            if (n0 + j < p.N) p.part_a[(part * p.N + n0 + j) * p.D + dch] = dA[j];
-    }
-    __syncthreads();
-    if (item) {
+        for (int k = 0; k < NG; ++k) raw_store<float, RN>(p.part_a + (part * p.D + dch) * p.N + n0(k), dA[k], count(k), p.vec_n);
+        wave_lds_fence();
 #pragma unroll
-        for (int i = 0; i < V; ++i) { s_dt[row * CPW + c0 + i] = d_skip[i]; s_du[row * CPW + c0 + i] = d_bias[i]; }
-    }
-    __syncthreads();
-    if (tid < CPW && c_first + tid < p.Dg) {
-        float x = 0.0f, y = 0.0f;
+        for (int i = 0; i < 4; ++i) { s_dt[(c0 + i) * kInLd + row] = d_skip[i]; s_du[(c0 + i) * kInLd + row] = d_bias[i]; }
+        wave_lds_fence();
+        if (lane < 16 && has) {
+            float x = 0.0f, y = 0.0f;
 #pragma unroll
-        for (int t = 0; t < kTile; ++t) { x += s_dt[t * CPW + tid]; y += s_du[t * CPW + tid]; }
-        p.part_d[part * p.D + g * p.Dg + c_first + tid] = x;
-        p.part_bias[part * p.D + g * p.Dg + c_first + tid] = y;
+            for (int t = 0; t < kTile; ++t) { x += s_dt[ch * kInLd + t]; y += s_du[ch * kInLd + t]; }
+            p.part_d[part * p.D + dch] = x;
+            p.part_bias[part * p.D + dch] = y;
+        }
     }
 }
 
-// Adds the parts up in a fixed order.  Workgroups 0 ... n_par - 1: 64 channels of one row of (dA: N rows, dD, ddt_bias), 16 threads a channel
-// over the parts; the others: 1024 elements of dB or dC over the channel blocks of their group.
+// Adds the parts up in a fixed order.  Workgroups 0 ... n_par - 1: 64 adjacent values of (dA [D][N], dD [D], ddt_bias [D]), 16 threads a value over
+// the parts; the others: 1024 elements of dB or dC over the channel blocks of their group.
 struct SsmFinishParams {
-    int B, T, D, N, G, nblk, parts, n_par, dblk;
+    int B, T, D, N, G, nblk, parts, n_par;
     const float *part_a, *part_d, *part_bias, *part_b, *part_c;
     float *dA, *dD, *ddt_bias;
     void *dB, *dC;
@@ -343,23 +405,24 @@ template <typename T>
 __global__ __launch_bounds__(1024) void ssm_finish_kernel(const SsmFinishParams p) {
     __shared__ float s_sum[16][64];
     if ((int)blockIdx.x < p.n_par) {
-        const int rowi = blockIdx.x / p.dblk, d = (blockIdx.x - rowi * p.dblk) * 64 + (threadIdx.x & 63), k = threadIdx.x >> 6;
-        const float* src = rowi < p.N ? p.part_a + (long long)rowi * p.D : rowi == p.N ? p.part_d : p.part_bias;
-        const long long step = rowi < p.N ? (long long)p.N * p.D : p.D;
+        const long long da = (long long)p.D * p.N, all = da + 2LL * p.D, i = (long long)blockIdx.x * 64 + (threadIdx.x & 63);
+        const int k = threadIdx.x >> 6;
+        const float* src = i < da ? p.part_a + i : i < da + p.D ? p.part_d + (i - da) : p.part_bias + (i - da - p.D);
+        const long long step = i < da ? da : p.D;
         float sum = 0.0f;
-        if (d < p.D) {
+        if (i < all) {
 #pragma unroll 8
-            for (int i = k; i < p.parts; i += 16) sum += src[i * step + d];
+            for (int j = k; j < p.parts; j += 16) sum += src[j * step];
         }
         s_sum[k][threadIdx.x & 63] = sum;
         __syncthreads();
-        if (threadIdx.x < 64 && d < p.D) {
+        if (threadIdx.x < 64 && i < all) {
             float t = 0.0f;
 #pragma unroll
-            for (int i = 0; i < 16; ++i) t += s_sum[i][threadIdx.x];
-            if (rowi < p.N) p.dA[(long long)d * p.N + rowi] = t;
-            else if (rowi == p.N) { if (p.dD) p.dD[d] = t; }
-            else if (p.ddt_bias) p.ddt_bias[d] = t;
+            for (int j = 0; j < 16; ++j) t += s_sum[j][threadIdx.x];
+            if (i < da) p.dA[i] = t;
+            else if (i < da + p.D) { if (p.dD) p.dD[i - da] = t; }
+            else if (p.ddt_bias) p.ddt_bias[i - da - p.D] = t;
         }
         return;
     }
@@ -404,25 +467,28 @@ static BwdLayout bwd_layout(const pcrl_ssm_desc* d, const SsmPlan& plan) {
     o.total = at * sizeof(float);
     return o;
 }
-size_t ssm_bwd_workspace(const pcrl_ssm_desc* d) { return bwd_layout(d, ssm_plan(d)).total; }
+size_t ssm_bwd_workspace(const pcrl_ssm_desc* d) { return bwd_layout(d, ssm_plan(d, true)).total; }
 
-template <typename T, int CPW>
+template <typename T, int RN, int NG, bool VEC>
 static int launch_bwd(const SsmParams& p, hipStream_t s) {
-    const int waves = ssm_waves(p.N), rows = 64 / CPW;
-    const size_t lds = sizeof(float) * kTile * CPW * (3 + (size_t)(p.z ? 3 : 2) * p.S * rows);
     const dim3 grid((unsigned)(p.G * p.nblk) * p.nchunk * (p.b_step < p.B ? p.b_step : p.B));
     if (p.nchunk > 1) {
-        ssm_bwd_kernel<T, CPW, true><<<grid, 64 * waves, sizeof(float) * kTile * CPW * 3, s>>>(p);
+        ssm_bwd_kernel<T, RN, NG, VEC, true><<<grid, 256, sizeof(float) * 4 * ssm_bwd_wave_lds<true>(), s>>>(p);
         PCRL_CHECK_LAUNCH("ssm_bwd_kernel (summary)");
     }
-    if (int rc = ensure_dynamic_lds((const void*)ssm_bwd_kernel<T, CPW, false>, lds)) return rc;
-    ssm_bwd_kernel<T, CPW, false><<<grid, 64 * waves, lds, s>>>(p);
+    const size_t lds = sizeof(float) * (4 * ssm_bwd_wave_lds<false>() + 4 * 2 * 16 * 4 * RN * NG);
+    if (int rc = ensure_dynamic_lds((const void*)ssm_bwd_kernel<T, RN, NG, VEC, false>, lds)) return rc;
+    ssm_bwd_kernel<T, RN, NG, VEC, false><<<grid, 256, lds, s>>>(p);
     PCRL_CHECK_LAUNCH("ssm_bwd_kernel");
     return PCRL_OK;
 }
+template <typename T, bool VEC>
+static int launch_bwd_n(const SsmParams& p, hipStream_t s) {
+    return p.N <= 4 ? launch_bwd<T, 1, 1, VEC>(p, s) : p.N <= 8 ? launch_bwd<T, 2, 1, VEC>(p, s) : p.N <= 16 ? launch_bwd<T, 4, 1, VEC>(p, s) : launch_bwd<T, 4, 2, VEC>(p, s);
+}
 template <typename T>
-static int launch_bwd_t(const SsmParams& p, int cpw, const SsmFinishParams& f, hipStream_t s) {
-    if (int rc = cpw == 64 ? launch_bwd<T, 64>(p, s) : cpw == 32 ? launch_bwd<T, 32>(p, s) : launch_bwd<T, 16>(p, s)) return rc;
+static int launch_bwd_t(const SsmParams& p, bool vec, const SsmFinishParams& f, hipStream_t s) {
+    if (int rc = vec ? launch_bwd_n<T, true>(p, s) : launch_bwd_n<T, false>(p, s)) return rc;
     const long long elems = 2LL * p.B * p.T * p.G * p.N;
     ssm_finish_kernel<T><<<dim3((unsigned)(f.n_par + (elems + 1023) / 1024)), 1024, 0, s>>>(f);
     PCRL_CHECK_LAUNCH("ssm_finish_kernel");
@@ -438,7 +504,8 @@ extern "C" int pcrl_ssm_scan_bwd(const pcrl_ssm_desc* d, const float* saved, con
     if (int rc = ssm_check(d, "pcrl_ssm_scan_bwd")) return rc;
     if (!saved || !dy || !g || !g->du || !g->ddt || !g->dB || !g->dC || !g->dA || (d->z && !g->dz))
         return fail(PCRL_E_ARG, "pcrl_ssm_scan_bwd: null saved state, gradient or output");
-    const SsmPlan plan = ssm_plan(d);
+    if (dy_st < 0 || dy_st >= (1LL << 26)) return fail(PCRL_E_ARG, "pcrl_ssm_scan_bwd: a step stride of %lld elements (0 to 2^26 - 1)", (long long)dy_st);
+    const SsmPlan plan = ssm_plan(d, true);
     const BwdLayout at = bwd_layout(d, plan);
     if (!workspace || workspace_bytes < at.total) return fail(PCRL_E_WORKSPACE, "pcrl_ssm_scan_bwd: workspace %zu < %zu", workspace_bytes, at.total);
     const long long elems = 2LL * d->B * d->T * d->G * d->N;
@@ -447,7 +514,7 @@ extern "C" int pcrl_ssm_scan_bwd(const pcrl_ssm_desc* d, const float* saved, con
     SsmParams p;
     ssm_fill(p, d);
     p.nblk = plan.nblk, p.nchunk = plan.nchunk, p.chunk_tiles = plan.chunk_tiles;
-    p.b_step = bwd_b_step(d, plan), p.parts = p.b_step * plan.nchunk;
+    p.b_step = bwd_b_step(d, plan);
     p.saved = const_cast<float*>(saved), p.dy = dy, p.dy_sb = dy_sb, p.dy_st = dy_st, p.dlast = dlast;
     p.du = g->du, p.ddt = g->ddt, p.dz = g->dz, p.dstate = g->dstate;
     p.part_b = w + at.b, p.part_c = w + at.c, p.part_a = w + at.a, p.part_d = w + at.dskip, p.part_bias = w + at.bias;
@@ -455,12 +522,14 @@ extern "C" int pcrl_ssm_scan_bwd(const pcrl_ssm_desc* d, const float* saved, con
     const void* extra[4] = {dy, g->du, g->ddt, g->dz};
     const long long dense[2] = {(long long)d->T * d->D, d->D};
     const long long strides[8] = {dy_sb, dy_st, dense[0], dense[1], dense[0], dense[1], dense[0], dense[1]};
-    p.vec = ssm_vec(d, plan.cpw / 16, extra, strides, 4);
+    const void* states[4] = {saved, dlast, g->dstate, workspace};
+    p.vec_n = ssm_vec_n(d, states, 4);
+    const bool vec = p.vec_n && ssm_vec(d, extra, strides, 4);
     SsmFinishParams f{};
-    f.B = d->B, f.T = d->T, f.D = d->D, f.N = d->N, f.G = d->G, f.nblk = plan.nblk, f.parts = p.parts;
-    f.dblk = cdiv(d->D, 64), f.n_par = (d->N + 2) * f.dblk;
+    f.B = d->B, f.T = d->T, f.D = d->D, f.N = d->N, f.G = d->G, f.nblk = plan.nblk, f.parts = p.b_step * plan.nchunk;
+    f.n_par = cdiv((long long)d->D * (d->N + 2), 64);
     f.part_a = p.part_a, f.part_d = p.part_d, f.part_bias = p.part_bias, f.part_b = p.part_b, f.part_c = p.part_c;
     f.dA = g->dA, f.dD = g->dD, f.ddt_bias = g->ddt_bias, f.dB = g->dB, f.dC = g->dC, f.lengths = d->lengths;
     hipStream_t s = (hipStream_t)stream;
-    return d->dtype == PCRL_DT_F32 ? launch_bwd_t<float>(p, plan.cpw, f, s) : d->dtype == PCRL_DT_BF16 ? launch_bwd_t<__bf16>(p, plan.cpw, f, s) : launch_bwd_t<_Float16>(p, plan.cpw, f, s);
+    return d->dtype == PCRL_DT_F32 ? launch_bwd_t<float>(p, vec, f, s) : d->dtype == PCRL_DT_BF16 ? launch_bwd_t<__bf16>(p, vec, f, s) : launch_bwd_t<_Float16>(p, vec, f, s);
 }

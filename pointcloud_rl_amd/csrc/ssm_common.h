@@ -1,11 +1,12 @@
 // Selective state space scan: what its forward (ssm_fwd.hip) and backward (ssm_bwd.hip) share.
 //
-// Work split.  A wave owns 4 of the N states of 64 channels, spread as CPW channels x (64 / CPW) state rows: with CPW = 64 a lane holds 4
-// states of one channel, with 32 two, with 16 one.  A workgroup is S = ceil(N / 4) such waves on the SAME CPW channels of one batch row (at
-// least 4 waves), so the recurrence runs without any exchange between lanes; B_t and C_t -- the same for every channel -- stand in a register
-// per state with step t0 + r in lane r of each 16-lane row, and reach the multiplies as DPP row broadcasts (no scalar loads, no LDS).
-// Steps go by tiles of 16: (1) the workgroup loads a 16 x CPW tile, one short vector per thread, forms dt and dt u once and leaves them in
-// LDS; (2) every wave walks the 16 steps for its states; (3) the waves' partial sums over the states are added up, gated and stored.
+// Work split.  A wave owns all states of 16 channels: lane = 16 q + c holds, of channel c, the RN = ceil(N / 4) states q RN ... q RN + RN - 1 (twice
+// that many in two groups for N > 16), so the recurrence runs without any exchange between lanes.  B_t and C_t -- the same for every channel --
+// stand in one register per state with step t0 + r in lane r of each 16-lane row, and reach the multiplies as DPP row broadcasts: no scalar
+// loads, no LDS.  Steps go by tiles of 16, all of it inside the wave (no workgroup barrier): (1) the 16 x 16 tile of every activation is loaded as
+// four adjacent channels per lane, dt and dt u are formed once per element and turned through LDS to four adjacent steps per lane; (2) the 16
+// steps are walked; (3) the four state rows' partial sums of each (step, channel) come back through LDS to the loading layout, where they are
+// added up, gated and stored.  A workgroup is four such waves on 64 adjacent channels: together they use whole cache lines.
 #pragma once
 #include "seq_common.h"
 
@@ -13,42 +14,47 @@ namespace pcrl {
 
 constexpr int kTile = 16;              // steps per tile = lanes of a DPP row
 constexpr int kSsmMaxN = 32;
+constexpr int kInLd = 20;              // [channel][step] tile in LDS: 16-byte reads of four steps, rows 4 banks apart
+constexpr int kInTile = 16 * kInLd;
+constexpr int kPartLd = 16 * 16 + 16;  // [state row][step][channel]: the four rows of a wave write to different banks
+constexpr int kPartTile = 4 * kPartLd;
 
 struct SsmParams {
     int B, T, D, N, G, Dg;             // Dg = D / G channels of a group
-    int S, nblk;                       // waves that hold states; channel blocks per group
-    int softplus, vec;                 // vec: every tensor admits whole-vector accesses
+    int nblk;                          // blocks of 64 channels per group
+    int softplus, vec_n;               // vec_n: the float states admit accesses of RN adjacent states
     int ntile, nchunk, chunk_tiles;    // tiles of the whole sequence; chunks it is cut into, tiles per chunk
     const void *u, *dt, *z, *Bm, *Cm, *dy;
     long long u_sb, u_st, dt_sb, dt_st, z_sb, z_st, b_sb, b_st, b_sg, c_sb, c_st, c_sg, dy_sb, dy_st;
     const float *A, *Dskip, *dt_bias, *state, *dlast;
     const uint8_t* starts; long long starts_sb;
     const int* lengths;
-    void* y; float* last; float* saved;            // saved [B][ntile][N][D]: the state in front of each tile
-    float* sum_p; float* sum_s;                    // chunk summaries [B][nchunk][N][D]: product of the decays, state from zero
+    void* y; float* last; float* saved;            // saved [B][ntile][D][N]: the state in front of each tile
+    float* sum_p; float* sum_s;                    // chunk summaries [B][nchunk][D][N]: product of the decays, state from zero
     // backward
     void *du, *ddt, *dz;
     float *part_b, *part_c;                        // [G * nblk][B][T][N]
-    float *part_a, *part_d, *part_bias;            // [parts][N][D], [parts][D]
+    float *part_a, *part_d, *part_bias;            // [parts][D][N], [parts][D]
     float* dstate;
-    int parts, b_step;                             // batch rows b, b + b_step, ... share a workgroup
+    int b_step;                                    // batch rows b, b + b_step, ... share a workgroup
 };
 
-// How a call is cut: channels per wave and chunks of the sequence.
-struct SsmPlan { int cpw, nblk, nchunk, chunk_tiles; };
+// How a call is cut into chunks.
+struct SsmPlan { int nblk, nchunk, chunk_tiles; };
 
 int ssm_check(const pcrl_ssm_desc* d, const char* who);
 void ssm_fill(SsmParams& p, const pcrl_ssm_desc* d);
-SsmPlan ssm_plan(const pcrl_ssm_desc* d);
-bool ssm_vec(const pcrl_ssm_desc* d, int V, const void* const* extra, const long long* strides, int n_extra);
-
-__host__ inline int ssm_waves(int N) { return N <= 16 ? 4 : (N + 3) / 4; }
+SsmPlan ssm_plan(const pcrl_ssm_desc* d, bool backward);
+// Whether every access admits whole vectors: four channels of the activations (the extra ones, with their two strides each, included), RN states
+// of B, C and the float states (the extra ones included).
+bool ssm_vec(const pcrl_ssm_desc* d, const void* const* extra, const long long* strides, int n_extra);
+bool ssm_vec_n(const pcrl_ssm_desc* d, const void* const* extra, int n_extra);
+__host__ inline int ssm_rn(int N) { return N <= 4 ? 1 : N <= 8 ? 2 : 4; }      // states per lane and group
 __host__ inline int cdiv(long long a, long long b) { return (int)((a + b - 1) / b); }
 
 #ifdef __HIPCC__
-// Where this workgroup works: the block index runs channel blocks fastest, then chunks, then batch rows.  Blocks go to the eight XCDs in turn;
-// when a row of channel blocks divides evenly, neighbouring blocks -- they read parts of the same cache lines and the same B_t, C_t -- are
-// dealt to one XCD.
+// Where this workgroup works: the block index runs channel blocks fastest, then chunks, then batch rows.  Workgroups go to the eight XCDs in
+// turn; when they divide evenly, neighbouring ones -- they read the same B_t and C_t -- are dealt to one XCD.
 __device__ __forceinline__ void ssm_where(const SsmParams& p, int& blk, int& chunk, int& b) {
     const unsigned n = gridDim.x;
     unsigned id = blockIdx.x;
@@ -68,6 +74,11 @@ __device__ __forceinline__ int ssm_length(const SsmParams& p, int b) {
 __device__ __forceinline__ unsigned ssm_start_bits(unsigned char mine) {
     const unsigned long long m = __ballot(mine != 0);
     return (unsigned)__builtin_amdgcn_readfirstlane((int)((unsigned)m & 0xFFFFu));
+}
+// Orders this wave's LDS writes before its LDS reads (LDS executes a wave's accesses in order: only the compiler has to be told).
+__device__ __forceinline__ void wave_lds_fence() {
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
 }
 #endif
 

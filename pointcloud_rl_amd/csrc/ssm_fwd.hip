@@ -1,179 +1,196 @@
 // Selective state space scan, forward and single step (ssm_common.h: the split; include/pcrl.h: the formulas).
 #include "ssm_common.h"
+#include <cstdlib>
 
 namespace pcrl {
 
 // SUMMARY: only the states are walked, from zero, and the chunk's summary (product of the decays, end state) is left; otherwise the chunk
 // starts from the combined summaries of the chunks in front of it and y is written.
-template <typename T, int CPW, bool SUMMARY>
-__global__ __launch_bounds__(512) void ssm_fwd_kernel(const SsmParams p) {
-    constexpr int NS = CPW / 16, V = CPW / 16, ROWS = 64 / CPW;       // states per lane, channels per thread, state rows per wave
-    extern __shared__ float lds[];
-    float* s_dt = lds;                                  // [16][CPW]
-    float* s_du = lds + kTile * CPW;                    // [16][CPW]
-    float* s_y = lds + 2 * kTile * CPW;                 // [S * ROWS][16][CPW]
-    const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
+template <typename T, int RN, int NG, bool VEC, bool SUMMARY>
+__global__ __launch_bounds__(256) void ssm_fwd_kernel(const SsmParams p) {
+    constexpr int kWave = 2 * kInTile + (SUMMARY ? 0 : kPartTile);
+    __shared__ float lds[4 * kWave];
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+    float* s_dt = lds + wave * kWave;                   // [channel][step]
+    float* s_du = s_dt + kInTile;
+    float* s_y = s_du + kInTile;                        // [state row][step][channel]: sum_n C h
     int blk, chunk, b;
     ssm_where(p, blk, chunk, b);
     if (SUMMARY && chunk == p.nchunk - 1) return;       // nobody starts from the last chunk's summary
-    const int g = blk / p.nblk, c_first = (blk - g * p.nblk) * CPW;   // first channel of this block inside its group
-    const int len = ssm_length(p, b);
+    const int g = blk / p.nblk, c_first = (blk - g * p.nblk) * 64 + wave * 16;        // first channel of this wave inside its group
+    const int left = p.Dg - c_first;                    // channels from there on
+    if (left <= 0) return;
+    const int len = ssm_length(p, b), d_first = g * p.Dg + c_first;
     const int tile0 = chunk * p.chunk_tiles, tile1 = tile0 + p.chunk_tiles < p.ntile ? tile0 + p.chunk_tiles : p.ntile;
 
-    // the thread's item of a tile: step `row`, channels c0 ... c0 + V - 1
-    const bool item = tid < 256;
-    const int row = (tid & 255) / 16, c0 = ((tid & 255) % 16) * V;
-    const int left = p.Dg - c_first - c0, nv = item ? (left < V ? left : V) : 0;
-    const int d0 = g * p.Dg + c_first + c0;             // global channel
-    float bias[V], skip[V];
+    // loading layout: step `row` of the tile, channels c0 ... c0 + 3 of the wave (clamped to what exists)
+    const int row = lane >> 2, c0 = (lane & 3) * 4, nv = left - c0 < 4 ? left - c0 : 4;
+    unsigned cc[4];
+    float bias[4], skip[4];
 #pragma unroll
-    for (int i = 0; i < V; ++i) {
-        bias[i] = i < nv && p.dt_bias ? p.dt_bias[d0 + i] : 0.0f;
-        skip[i] = i < nv && p.Dskip ? p.Dskip[d0 + i] : 0.0f;
+    for (int i = 0; i < 4; ++i) {
+        cc[i] = c0 + i < left ? c0 + i : (VEC ? 0 : left - 1);
+        bias[i] = i < nv && p.dt_bias ? p.dt_bias[d_first + c0 + i] : 0.0f;
+        skip[i] = i < nv && p.Dskip ? p.Dskip[d_first + c0 + i] : 0.0f;
     }
-    const T* pu = (const T*)p.u + b * p.u_sb + d0;
-    const T* pd = (const T*)p.dt + b * p.dt_sb + d0;
-    const T* pz = p.z ? (const T*)p.z + b * p.z_sb + d0 : nullptr;
-    T* py = (T*)p.y + ((long long)b * p.T) * p.D + d0;
+    const T* pu = (const T*)p.u + b * p.u_sb + d_first;
+    const T* pd = (const T*)p.dt + b * p.dt_sb + d_first;
+    const T* pz = p.z ? (const T*)p.z + b * p.z_sb + d_first : nullptr;
+    T* py = (T*)p.y + (long long)b * p.T * p.D + d_first;
 
-    // the lane's states: channel `ch` of the block, states n0 ... n0 + NS - 1
-    const int ch = lane % CPW, n0 = wave * 4 + (lane / CPW) * NS;
-    const int dch = g * p.Dg + c_first + ch;
-    const bool has = c_first + ch < p.Dg;
-    const bool walks = wave < p.S;
-    float A2[NS], h[NS];
+    // walking layout: channel ch of the wave, states n0(k) ... n0(k) + RN - 1 of group k
+    const int ch = lane & 15, q = lane >> 4, dch = d_first + ch;
+    const bool has = ch < left;
+    auto n0 = [&](int k) { return (k * 4 + q) * RN; };
+    auto count = [&](int k) { const int n = p.N - n0(k); return has ? (n < RN ? n : RN) : 0; };
+    unsigned nn[NG][RN];
+    float A2[NG][RN], h[NG][RN];
 #pragma unroll
-    for (int j = 0; j < NS; ++j) {
-        const bool on = walks && has && n0 + j < p.N;
-        A2[j] = on ? p.A[(long long)dch * p.N + n0 + j] * kLog2e : 0.0f;
-        h[j] = !SUMMARY && on && p.state ? p.state[((long long)b * p.D + dch) * p.N + n0 + j] : 0.0f;
-    }
-    if (!SUMMARY && walks && has) {                     // h = P h + S over the chunks in front
-        for (int c = 0; c < chunk; ++c) {
+    for (int k = 0; k < NG; ++k) {
+        const RawVec<float, RN> a = raw_load<float, RN>(p.A + (long long)dch * p.N + n0(k), count(k), p.vec_n);
+        const RawVec<float, RN> s = raw_load<float, RN>(p.state + ((long long)b * p.D + dch) * p.N + n0(k), !SUMMARY && p.state ? count(k) : 0, p.vec_n);
 #pragma unroll
-            for (int j = 0; j < NS; ++j)
-                if (n0 + j < p.N) {
-                    const long long at = (((long long)b * p.nchunk + c) * p.N + n0 + j) * p.D + dch;
-                    const float P = p.sum_p[at], s = p.sum_s[at];
-                    h[j] = P == 0.0f ? s : __builtin_fmaf(P, h[j], s);
-                }
+        for (int j = 0; j < RN; ++j) {
+            A2[k][j] = a.v[j] * kLog2e;
+            h[k][j] = s.v[j];
+            nn[k][j] = n0(k) + j < p.N ? n0(k) + j : (VEC ? 0 : p.N - 1);
+        }
+        if (!SUMMARY) {                                 // h = P h + S over the chunks in front
+            for (int c = 0; c < chunk; ++c) {
+                const long long at = (((long long)b * p.nchunk + c) * p.D + dch) * p.N + n0(k);
+                const RawVec<float, RN> P = raw_load<float, RN>(p.sum_p + at, count(k), p.vec_n), S = raw_load<float, RN>(p.sum_s + at, count(k), p.vec_n);
+#pragma unroll
+                for (int j = 0; j < RN; ++j) h[k][j] = P.v[j] == 0.0f ? S.v[j] : __builtin_fmaf(P.v[j], h[k][j], S.v[j]);
+            }
         }
     }
     const T* pB = (const T*)p.Bm + b * p.b_sb + g * p.b_sg;
     const T* pC = (const T*)p.Cm + b * p.c_sb + g * p.c_sg;
     const uint8_t* ps = p.starts ? p.starts + b * p.starts_sb : nullptr;
+    const bool clean = left >= 16 && p.N == 4 * RN * NG;              // every lane's channels and states exist
     float dt_sum = 0.0f;
     bool cut = false;                                   // a start inside the chunk: nothing from before reaches its end
 
-    RawVec<T, V> nu, nd, nz;
-    T nB[NS], nC[NS];
-    unsigned char nst;
-    auto fetch = [&](int tile) {
-        const int t = tile * kTile + row, n = t < len ? nv : 0;
-        nu = raw_load<T, V>(pu + t * p.u_st, n, p.vec);
-        nd = raw_load<T, V>(pd + t * p.dt_st, n, p.vec);
-        if (!SUMMARY && pz) nz = raw_load<T, V>(pz + t * p.z_st, n, p.vec);
-        const int tl = tile * kTile + (lane & 15);
-        const bool on = walks && tl < len;
+    RawVec<T, 4> nu, nd, nz;
+    RawVec<T, RN> nB[NG], nC[NG];
+    unsigned nst = 0;
+    auto fetch = [&](int tile) {                        // rows behind the length read the last one
+        const long long t0 = (long long)tile * kTile;
+        const int last = len - 1 - (int)t0, r = row < last ? row : last, rn = ch < last ? ch : last;
+        nu = lane_load<T, 4, VEC>(pu + t0 * p.u_st, r * (unsigned)p.u_st, cc);
+        nd = lane_load<T, 4, VEC>(pd + t0 * p.dt_st, r * (unsigned)p.dt_st, cc);
+        if (!SUMMARY && pz) nz = lane_load<T, 4, VEC>(pz + t0 * p.z_st, r * (unsigned)p.z_st, cc);
 #pragma unroll
-        for (int j = 0; j < NS; ++j) {
-            nB[j] = on && n0 + j < p.N ? pB[tl * p.b_st + n0 + j] : (T)0.0f;
-            if (!SUMMARY) nC[j] = on && n0 + j < p.N ? pC[tl * p.c_st + n0 + j] : (T)0.0f;
+        for (int k = 0; k < NG; ++k) {                  // lane r of a 16-lane row: step r
+            nB[k] = lane_load<T, RN, VEC>(pB + t0 * p.b_st, rn * (unsigned)p.b_st, nn[k]);
+            if (!SUMMARY) nC[k] = lane_load<T, RN, VEC>(pC + t0 * p.c_st, rn * (unsigned)p.c_st, nn[k]);
         }
-        nst = ps && tl < len ? ps[tl] : (unsigned char)0;
+        if (ps) nst = ch <= last ? ps[t0 + rn] : 0;
     };
     const int live = (len + kTile - 1) / kTile, end = tile1 < live ? tile1 : live;      // tiles with a step in them
     if (tile0 < end) fetch(tile0);
     for (int tile = tile0; tile < end; ++tile) {
         const int t0 = tile * kTile;
-        float u[V], z[V], Bv[NS], Cv[NS];
-        const bool here = t0 + row < len;
-        {
-            float dt[V], du[V];
+        const bool plain = clean && t0 + kTile <= len, here = t0 + row < len;
+        float u[4], z[4], Bv[NG][RN], Cv[NG][RN];
+        float dt[4];
 #pragma unroll
-            for (int i = 0; i < V; ++i) {
-                u[i] = (float)nu.v[i];
-                z[i] = !SUMMARY && pz ? (float)nz.v[i] : 0.0f;
-                float slope;
-                const float raw = (float)nd.v[i] + bias[i];
-                dt[i] = p.softplus ? softplus_(raw, slope) : raw;
-                dt[i] = here ? dt[i] : 0.0f;            // a step behind the length changes nothing: decay 1, input 0
-                du[i] = dt[i] * u[i];
-            }
-            if (item) {
-#pragma unroll
-                for (int i = 0; i < V; ++i) { s_dt[row * CPW + c0 + i] = dt[i]; s_du[row * CPW + c0 + i] = du[i]; }
-            }
+        for (int i = 0; i < 4; ++i) {
+            u[i] = (float)nu.v[i];
+            z[i] = !SUMMARY && pz ? (float)nz.v[i] : 0.0f;
+            float slope;
+            const float raw = (float)nd.v[i] + bias[i];
+            dt[i] = p.softplus ? softplus_(raw, slope) : raw;
         }
 #pragma unroll
-        for (int j = 0; j < NS; ++j) { Bv[j] = (float)nB[j]; Cv[j] = !SUMMARY ? (float)nC[j] : 0.0f; }
-        const unsigned starts = ssm_start_bits(nst);
-        if (tile + 1 < end) fetch(tile + 1);
-        __syncthreads();
-        if (walks) {
-            if (!SUMMARY && p.saved && has) {
+        for (int k = 0; k < NG; ++k)
 #pragma unroll
-                for (int j = 0; j < NS; ++j)
-                    if (n0 + j < p.N) p.saved[(((long long)b * p.ntile + tile) * p.N + n0 + j) * p.D + dch] = h[j];
+            for (int j = 0; j < RN; ++j) { Bv[k][j] = (float)nB[k].v[j]; Cv[k][j] = !SUMMARY ? (float)nC[k].v[j] : 0.0f; }
+        if (!plain) {                                   // a step behind the length changes nothing: decay 1, input 0
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                dt[i] = here ? dt[i] : 0.0f;
+                u[i] = here ? u[i] : 0.0f;
             }
-            float* out = s_y + (wave * ROWS + lane / CPW) * (kTile * CPW) + ch;
-            auto walk = [&](auto with_starts) {
-                static_for<kTile>([&](auto ti) {
-                    constexpr int t = decltype(ti)::value;
-                    const float dt = s_dt[t * CPW + ch], du = s_du[t * CPW + ch];
+#pragma unroll
+            for (int k = 0; k < NG; ++k)
+#pragma unroll
+                for (int j = 0; j < RN; ++j) {
+                    const bool on = t0 + ch < len && n0(k) + j < p.N;
+                    Bv[k][j] = on ? Bv[k][j] : 0.0f;
+                    Cv[k][j] = on ? Cv[k][j] : 0.0f;
+                }
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            s_dt[(c0 + i) * kInLd + row] = dt[i];
+            s_du[(c0 + i) * kInLd + row] = dt[i] * u[i];
+        }
+        const unsigned starts = ps ? ssm_start_bits(nst) : 0u;
+        wave_lds_fence();
+        if (tile + 1 < end) fetch(tile + 1);
+        if (!SUMMARY && p.saved) {
+            float* at = p.saved + (((long long)b * p.ntile + tile) * p.D + d_first) * p.N;
+#pragma unroll
+            for (int k = 0; k < NG; ++k) lane_store<float, RN, VEC>(at, ch * (unsigned)p.N + n0(k), h[k], count(k));
+        }
+        auto walk = [&](auto with_starts) {
+            static_for<4>([&](auto gi) {
+                constexpr int tg = decltype(gi)::value * 4;
+                const f32x4 dt4 = *(const f32x4*)(s_dt + ch * kInLd + tg), du4 = *(const f32x4*)(s_du + ch * kInLd + tg);
+                static_for<4>([&](auto ti) {
+                    constexpr int i = decltype(ti)::value, t = tg + i;
                     const bool fresh = decltype(with_starts)::value && ((starts >> t) & 1u);
                     float acc = 0.0f;
 #pragma unroll
-                    for (int j = 0; j < NS; ++j) {
-                        const float x = du * row_bcast<t>(Bv[j]);
-                        const float a = __builtin_amdgcn_exp2f(dt * A2[j]);
-                        const float hn = __builtin_fmaf(a, h[j], x);
-                        h[j] = fresh ? x : hn;
-                        if (!SUMMARY) acc = j == 0 ? h[j] * row_bcast<t>(Cv[j]) : __builtin_fmaf(row_bcast<t>(Cv[j]), h[j], acc);
+                    for (int k = 0; k < NG; ++k) {
+#pragma unroll
+                        for (int j = 0; j < RN; ++j) {
+                            const float x = du4[i] * row_bcast<t>(Bv[k][j]);
+                            const float hn = __builtin_fmaf(__builtin_amdgcn_exp2f(dt4[i] * A2[k][j]), h[k][j], x);
+                            h[k][j] = fresh ? x : hn;
+                        }
+                        if (!SUMMARY) dot_row_bcast<t, RN>(acc, Cv[k], h[k]);
                     }
-                    if (SUMMARY) dt_sum += dt;
-                    else out[t * CPW] = acc;
+                    if (SUMMARY) dt_sum += dt4[i];
+                    else s_y[q * kPartLd + t * 16 + ch] = acc;
                 });
-            };
-            if (starts) { walk(std::true_type{}); cut = true; }
-            else walk(std::false_type{});
-        }
-        __syncthreads();
-        if (!SUMMARY && item) {
-            float acc[V];
+            });
+        };
+        if (starts) { walk(std::true_type{}); cut = true; }
+        else walk(std::false_type{});
+        wave_lds_fence();
+        if (!SUMMARY) {
+            f32x4 s = *(const f32x4*)(s_y + row * 16 + c0);
 #pragma unroll
-            for (int i = 0; i < V; ++i) acc[i] = 0.0f;
-            for (int s = 0; s < p.S * ROWS; ++s)
+            for (int k = 1; k < 4; ++k) s += *(const f32x4*)(s_y + k * kPartLd + row * 16 + c0);
+            float out[4];
 #pragma unroll
-                for (int i = 0; i < V; ++i) acc[i] += s_y[s * (kTile * CPW) + row * CPW + c0 + i];
-#pragma unroll
-            for (int i = 0; i < V; ++i) {
-                acc[i] = __builtin_fmaf(skip[i], u[i], acc[i]);
-                if (pz) acc[i] *= z[i] * sigmoidf_(z[i]);
-                acc[i] = here ? acc[i] : 0.0f;
+            for (int i = 0; i < 4; ++i) {
+                out[i] = __builtin_fmaf(skip[i], u[i], s[i]);
+                if (pz) out[i] *= z[i] * sigmoidf_(z[i]);
+                if (!plain) out[i] = here ? out[i] : 0.0f;
             }
-            raw_store<T, V>(py + (long long)(t0 + row) * p.D, acc, t0 + row < p.T ? nv : 0, p.vec);
+            lane_store<T, 4, VEC>(py + (long long)t0 * p.D, row * (unsigned)p.D + c0, out, t0 + row < p.T ? nv : 0);
         }
     }
     if (!SUMMARY) {                                     // steps behind the length: zeros
-        float none[V];
-#pragma unroll
-        for (int i = 0; i < V; ++i) none[i] = 0.0f;
+        const float none[4] = {0.0f, 0.0f, 0.0f, 0.0f};
         for (int tile = tile0 > live ? tile0 : live; tile < tile1; ++tile)
-            raw_store<T, V>(py + (long long)(tile * kTile + row) * p.D, none, tile * kTile + row < p.T ? nv : 0, p.vec);
+            lane_store<T, 4, VEC>(py + (long long)tile * kTile * p.D, row * (unsigned)p.D + c0, none, tile * kTile + row < p.T ? nv : 0);
     }
-    if (walks && has) {
 #pragma unroll
-        for (int j = 0; j < NS; ++j)
-            if (n0 + j < p.N) {
-                if (SUMMARY) {
-                    const long long at = (((long long)b * p.nchunk + chunk) * p.N + n0 + j) * p.D + dch;
-                    p.sum_p[at] = cut ? 0.0f : __builtin_amdgcn_exp2f(dt_sum * A2[j]);
-                    p.sum_s[at] = h[j];
-                } else if (p.last && chunk == p.nchunk - 1) {
-                    p.last[((long long)b * p.D + dch) * p.N + n0 + j] = h[j];
-                }
-            }
+    for (int k = 0; k < NG; ++k) {
+        if (SUMMARY) {
+            const long long at = (((long long)b * p.nchunk + chunk) * p.D + dch) * p.N + n0(k);
+            float P[RN];
+#pragma unroll
+            for (int j = 0; j < RN; ++j) P[j] = cut ? 0.0f : __builtin_amdgcn_exp2f(dt_sum * A2[k][j]);
+            raw_store<float, RN>(p.sum_p + at, P, count(k), p.vec_n);
+            raw_store<float, RN>(p.sum_s + at, h[k], count(k), p.vec_n);
+        } else if (p.last && chunk == p.nchunk - 1) {
+            raw_store<float, RN>(p.last + ((long long)b * p.D + dch) * p.N + n0(k), h[k], count(k), p.vec_n);
+        }
     }
 }
 
@@ -230,14 +247,36 @@ int ssm_check(const pcrl_ssm_desc* d, const char* who) {
     if (d->N > kSsmMaxN) return fail(PCRL_E_ARG, "%s: N = %d states per channel (at most %d)", who, d->N, kSsmMaxN);
     if (d->D % d->G) return fail(PCRL_E_ARG, "%s: %d channels are not shared evenly by %d groups", who, d->D, d->G);
     if (!seq_dtype(d->dtype)) return fail(PCRL_E_ARG, "%s: dtype %d", who, d->dtype);
+    for (long long st : {d->u_st, d->dt_st, d->z_st, d->b_st, d->c_st})        // offsets inside a tile of 16 steps are 32-bit
+        if (st < 0 || st >= (1LL << 26)) return fail(PCRL_E_ARG, "%s: a step stride of %lld elements (0 to 2^26 - 1)", who, st);
+    if (d->D >= (1 << 26)) return fail(PCRL_E_ARG, "%s: D = %d", who, d->D);
     if (!d->u || !d->dt || !d->Bm || !d->Cm || !d->A) return fail(PCRL_E_ARG, "%s: null input", who);
     return PCRL_OK;
+}
+
+bool ssm_vec(const pcrl_ssm_desc* d, const void* const* extra, const long long* strides, int n_extra) {
+    const size_t bytes = 4 * (size_t)elem_bytes(d->dtype);
+    if ((d->D / d->G) % 4) return false;
+    const void* ptr[3] = {d->u, d->dt, d->z};
+    const long long st[3][2] = {{d->u_sb, d->u_st}, {d->dt_sb, d->dt_st}, {d->z_sb, d->z_st}};
+    for (int i = 0; i < 3; ++i)
+        if (ptr[i] && ((uintptr_t)ptr[i] % bytes || st[i][0] % 4 || st[i][1] % 4)) return false;
+    for (int i = 0; i < n_extra; ++i)
+        if (extra[i] && ((uintptr_t)extra[i] % bytes || strides[2 * i] % 4 || strides[2 * i + 1] % 4)) return false;
+    const int rn = ssm_rn(d->N);
+    return d->N % rn == 0 && ((uintptr_t)d->Bm | (uintptr_t)d->Cm) % ((uintptr_t)rn * elem_bytes(d->dtype)) == 0 &&
+           (d->b_sb | d->b_st | d->b_sg | d->c_sb | d->c_st | d->c_sg) % rn == 0;
+}
+bool ssm_vec_n(const pcrl_ssm_desc* d, const void* const* extra, int n_extra) {
+    const int rn = ssm_rn(d->N);
+    uintptr_t all = (uintptr_t)d->A | (uintptr_t)d->state;
+    for (int i = 0; i < n_extra; ++i) all |= (uintptr_t)extra[i];
+    return d->N % rn == 0 && all % (4 * (uintptr_t)rn) == 0;
 }
 
 void ssm_fill(SsmParams& p, const pcrl_ssm_desc* d) {
     p = SsmParams{};
     p.B = d->B, p.T = d->T, p.D = d->D, p.N = d->N, p.G = d->G, p.Dg = d->D / d->G;
-    p.S = cdiv(d->N, 4);
     p.softplus = d->softplus != 0;
     p.ntile = cdiv(d->T, kTile);
     p.u = d->u, p.dt = d->dt, p.z = d->z, p.Bm = d->Bm, p.Cm = d->Cm;
@@ -247,59 +286,43 @@ void ssm_fill(SsmParams& p, const pcrl_ssm_desc* d) {
     p.starts = d->starts, p.starts_sb = d->starts_sb, p.lengths = d->lengths;
 }
 
-// Whole-vector accesses: V channels of every row start at a multiple of V elements.
-bool ssm_vec(const pcrl_ssm_desc* d, int V, const void* const* extra, const long long* strides, int n_extra) {
-    const size_t bytes = (size_t)V * elem_bytes(d->dtype);
-    if ((d->D / d->G) % V) return false;
-    const void* ptr[3] = {d->u, d->dt, d->z};
-    const long long st[3][2] = {{d->u_sb, d->u_st}, {d->dt_sb, d->dt_st}, {d->z_sb, d->z_st}};
-    for (int i = 0; i < 3; ++i) {
-        if (!ptr[i]) continue;
-        if ((uintptr_t)ptr[i] % bytes || st[i][0] % V || st[i][1] % V) return false;
-    }
-    for (int i = 0; i < n_extra; ++i) {
-        if (!extra[i]) continue;
-        if ((uintptr_t)extra[i] % bytes || strides[2 * i] % V || strides[2 * i + 1] % V) return false;
-    }
-    return true;
-}
-
-SsmPlan ssm_plan(const pcrl_ssm_desc* d) {
-    const int Dg = d->D / d->G, ntile = cdiv(d->T, kTile);
-    const long long cus = num_cus();
+SsmPlan ssm_plan(const pcrl_ssm_desc* d, bool backward) {
     SsmPlan plan{};
-    for (int cpw = 64; cpw >= 16; cpw >>= 1) {
-        plan.cpw = cpw, plan.nblk = cdiv(Dg, cpw);
-        if ((long long)d->B * d->G * plan.nblk >= cus) break;
-    }
-    const long long blocks = (long long)d->B * d->G * plan.nblk, want = 8 * cus / blocks;
-    const int most = ntile / 8 < 1 ? 1 : ntile / 8;
-    const int chunks = want < 4 || most < 4 ? 1 : want < most ? (int)want : most;
+    const int ntile = cdiv(d->T, kTile);
+    plan.nblk = cdiv(d->D / d->G, 64);
+    const long long blocks = (long long)d->B * d->G * plan.nblk;
+    long long chunks = 4LL * num_cus() / blocks;
+    const char* e = getenv(backward ? "PCRL_X_BCHUNKS" : "PCRL_X_CHUNKS");
+    if (e) chunks = atoi(e);
+    if (chunks > ntile / 2) chunks = ntile / 2;
+    if (chunks < 2) chunks = 1;
     plan.chunk_tiles = cdiv(ntile, chunks);
     plan.nchunk = cdiv(ntile, plan.chunk_tiles);
     return plan;
 }
 
-template <typename T, int CPW>
-static int launch_fwd(SsmParams& p, hipStream_t s) {
-    const int waves = ssm_waves(p.N), rows = 64 / CPW;
-    const size_t lds = sizeof(float) * kTile * CPW * (2 + (size_t)p.S * rows);
+template <typename T, int RN, int NG, bool VEC>
+static int launch_fwd(const SsmParams& p, hipStream_t s) {
+    const dim3 grid((unsigned)(p.G * p.nblk) * p.nchunk * p.B);
     if (p.nchunk > 1) {
-        ssm_fwd_kernel<T, CPW, true><<<dim3((unsigned)(p.G * p.nblk) * p.nchunk * p.B), 64 * waves, sizeof(float) * kTile * CPW * 2, s>>>(p);
+        ssm_fwd_kernel<T, RN, NG, VEC, true><<<grid, 256, 0, s>>>(p);
         PCRL_CHECK_LAUNCH("ssm_fwd_kernel (summary)");
     }
-    ssm_fwd_kernel<T, CPW, false><<<dim3((unsigned)(p.G * p.nblk) * p.nchunk * p.B), 64 * waves, lds, s>>>(p);
+    ssm_fwd_kernel<T, RN, NG, VEC, false><<<grid, 256, 0, s>>>(p);
     PCRL_CHECK_LAUNCH("ssm_fwd_kernel");
     return PCRL_OK;
 }
+template <typename T, bool VEC>
+static int launch_fwd_n(const SsmParams& p, hipStream_t s) {
+    return p.N <= 4 ? launch_fwd<T, 1, 1, VEC>(p, s) : p.N <= 8 ? launch_fwd<T, 2, 1, VEC>(p, s) : p.N <= 16 ? launch_fwd<T, 4, 1, VEC>(p, s) : launch_fwd<T, 4, 2, VEC>(p, s);
+}
 template <typename T>
-static int launch_fwd_t(SsmParams& p, int cpw, hipStream_t s) {
-    return cpw == 64 ? launch_fwd<T, 64>(p, s) : cpw == 32 ? launch_fwd<T, 32>(p, s) : launch_fwd<T, 16>(p, s);
-}
+static int launch_fwd_t(const SsmParams& p, bool vec, hipStream_t s) { return vec ? launch_fwd_n<T, true>(p, s) : launch_fwd_n<T, false>(p, s); }
 
-static size_t fwd_workspace(const pcrl_ssm_desc* d, const SsmPlan& plan) {
-    return plan.nchunk > 1 ? sizeof(float) * 2 * (size_t)d->B * plan.nchunk * d->N * d->D : 0;
+static size_t fwd_summary(const pcrl_ssm_desc* d, const SsmPlan& plan) {                 // floats, a multiple of 16 bytes
+    return plan.nchunk > 1 ? ((size_t)d->B * plan.nchunk * d->N * d->D + 3) & ~(size_t)3 : 0;
 }
+static size_t fwd_workspace(const pcrl_ssm_desc* d, const SsmPlan& plan) { return sizeof(float) * 2 * fwd_summary(d, plan); }
 size_t ssm_bwd_workspace(const pcrl_ssm_desc* d);       // ssm_bwd.hip
 
 }  // namespace pcrl
@@ -308,7 +331,7 @@ using namespace pcrl;
 
 extern "C" int pcrl_ssm_scan_bytes(const pcrl_ssm_desc* d, size_t* workspace, size_t* saved, size_t* bwd) {
     if (int rc = ssm_check(d, "pcrl_ssm_scan_bytes")) return rc;
-    if (workspace) *workspace = fwd_workspace(d, ssm_plan(d));
+    if (workspace) *workspace = fwd_workspace(d, ssm_plan(d, false));
     if (saved) *saved = sizeof(float) * (size_t)d->B * cdiv(d->T, kTile) * d->N * d->D;
     if (bwd) *bwd = ssm_bwd_workspace(d);
     return PCRL_OK;
@@ -317,7 +340,7 @@ extern "C" int pcrl_ssm_scan_bytes(const pcrl_ssm_desc* d, size_t* workspace, si
 extern "C" int pcrl_ssm_scan_fwd(const pcrl_ssm_desc* d, void* y, float* last_state, float* saved, void* workspace, size_t workspace_bytes, void* stream) {
     if (int rc = ssm_check(d, "pcrl_ssm_scan_fwd")) return rc;
     if (!y) return fail(PCRL_E_ARG, "pcrl_ssm_scan_fwd: null output");
-    const SsmPlan plan = ssm_plan(d);
+    const SsmPlan plan = ssm_plan(d, false);
     const size_t need = fwd_workspace(d, plan);
     if (need && (!workspace || workspace_bytes < need)) return fail(PCRL_E_WORKSPACE, "pcrl_ssm_scan_fwd: workspace %zu < %zu", workspace_bytes, need);
     if ((long long)d->G * plan.nblk * plan.nchunk * d->B > 0x7FFFFFFFLL) return fail(PCRL_E_ARG, "pcrl_ssm_scan_fwd: too many workgroups");
@@ -325,12 +348,14 @@ extern "C" int pcrl_ssm_scan_fwd(const pcrl_ssm_desc* d, void* y, float* last_st
     ssm_fill(p, d);
     p.nblk = plan.nblk, p.nchunk = plan.nchunk, p.chunk_tiles = plan.chunk_tiles;
     p.y = y, p.last = last_state, p.saved = saved;
-    p.sum_p = (float*)workspace, p.sum_s = p.sum_p + (size_t)d->B * plan.nchunk * d->N * d->D;
+    p.sum_p = (float*)workspace, p.sum_s = p.sum_p + fwd_summary(d, plan);
     const void* extra[1] = {y};
     const long long strides[2] = {(long long)d->T * d->D, d->D};
-    p.vec = ssm_vec(d, plan.cpw / 16, extra, strides, 1);
+    const void* states[3] = {last_state, saved, workspace};
+    p.vec_n = ssm_vec_n(d, states, 3);
+    const bool vec = p.vec_n && ssm_vec(d, extra, strides, 1);
     hipStream_t s = (hipStream_t)stream;
-    return d->dtype == PCRL_DT_F32 ? launch_fwd_t<float>(p, plan.cpw, s) : d->dtype == PCRL_DT_BF16 ? launch_fwd_t<__bf16>(p, plan.cpw, s) : launch_fwd_t<_Float16>(p, plan.cpw, s);
+    return d->dtype == PCRL_DT_F32 ? launch_fwd_t<float>(p, vec, s) : d->dtype == PCRL_DT_BF16 ? launch_fwd_t<__bf16>(p, vec, s) : launch_fwd_t<_Float16>(p, vec, s);
 }
 
 extern "C" int pcrl_ssm_step(const pcrl_ssm_desc* d, void* y, float* state_out, void* stream) {
