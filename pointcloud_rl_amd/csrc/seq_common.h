@@ -105,7 +105,7 @@ __device__ __forceinline__ float row_bcast(float v) {
     return u2f((unsigned)__builtin_amdgcn_update_dpp(0, (int)f2u(v), 0x150 + I, 0xF, 0xF, true));
 }
 
-// acc[j] += (lane I of the row of c[j]) * x, and acc += sum_j (lane I of the row of c[j]) * x[j].  The compiler folds a row broadcast into a
+// acc[j] += (lane I of the row of c[j]) * x, and the sum over j of (lane I of the row of c[j]) * x[j].  The compiler folds a row broadcast into a
 // multiply but not into a multiply-add.  s_nop 1: the two wait states between a vector instruction that may have written c and the DPP read of
 // it, whatever stands in front.
 #define PCRL_FMAC_ROW(ACC, C, X, I) "v_fmac_f32_dpp %" #ACC ", %" #C ", %" #X " row_newbcast:%" #I " row_mask:0xf bank_mask:0xf\n\t"
@@ -120,14 +120,14 @@ __device__ __forceinline__ void fma_row_bcast(float (&acc)[RN], const float (&c)
         asm("s_nop 1\n\t" PCRL_FMAC_ROW(0, 1, 2, 3) : "+v"(acc[0]) : "v"(c[0]), "v"(x), "n"(I));
 }
 template <int I, int RN>
-__device__ __forceinline__ void dot_row_bcast(float& acc, const float (&c)[RN], const float (&x)[RN]) {
+__device__ __forceinline__ float dot_row_bcast(const float (&c)[RN], const float (&x)[RN]) {
+    float acc = x[0] * row_bcast<I>(c[0]);
     if constexpr (RN == 4)
-        asm("s_nop 1\n\t" PCRL_FMAC_ROW(0, 1, 5, 9) PCRL_FMAC_ROW(0, 2, 6, 9) PCRL_FMAC_ROW(0, 3, 7, 9) PCRL_FMAC_ROW(0, 4, 8, 9)
-            : "+v"(acc) : "v"(c[0]), "v"(c[1]), "v"(c[2]), "v"(c[3]), "v"(x[0]), "v"(x[1]), "v"(x[2]), "v"(x[3]), "n"(I));
+        asm("s_nop 1\n\t" PCRL_FMAC_ROW(0, 1, 4, 7) PCRL_FMAC_ROW(0, 2, 5, 7) PCRL_FMAC_ROW(0, 3, 6, 7)
+            : "+v"(acc) : "v"(c[1]), "v"(c[2]), "v"(c[3]), "v"(x[1]), "v"(x[2]), "v"(x[3]), "n"(I));
     else if constexpr (RN == 2)
-        asm("s_nop 1\n\t" PCRL_FMAC_ROW(0, 1, 3, 5) PCRL_FMAC_ROW(0, 2, 4, 5) : "+v"(acc) : "v"(c[0]), "v"(c[1]), "v"(x[0]), "v"(x[1]), "n"(I));
-    else
-        asm("s_nop 1\n\t" PCRL_FMAC_ROW(0, 1, 2, 3) : "+v"(acc) : "v"(c[0]), "v"(x[0]), "n"(I));
+        asm("s_nop 1\n\t" PCRL_FMAC_ROW(0, 1, 2, 3) : "+v"(acc) : "v"(c[1]), "v"(x[1]), "n"(I));
+    return acc;
 }
 #undef PCRL_FMAC_ROW
 

@@ -73,15 +73,17 @@ __device__ __forceinline__ void fold_step(const float (&v)[RN], float (&held)[4]
     }
 }
 
-// LDS per wave, in floats: the three [channel][step] tiles, softplus slopes of the loading layout, three [state row][step][channel] partial sums.
-template <bool SUMMARY> constexpr int ssm_bwd_wave_lds() { return SUMMARY ? 2 * kInTile : 3 * kInTile + 256 + 3 * kPartTile; }
+// LDS per wave, in floats: dt_bias and D of its channels, the three [channel][step] tiles, softplus slopes of the loading layout, three [state row][step][channel] partial sums.
+template <bool SUMMARY> constexpr int ssm_bwd_wave_lds() { return SUMMARY ? 32 + 2 * kInTile : 32 + 3 * kInTile + 256 + 3 * kPartTile; }
 
 template <typename T, int RN, int NG, bool VEC, bool SUMMARY>
-__global__ __launch_bounds__(256, 2) void ssm_bwd_kernel(const SsmParams p) {
+__global__ __launch_bounds__(256, 2) void ssm_bwd_kernel(const SsmParams) {
+    const SsmArgs p = ssm_args();
     constexpr int kWave = ssm_bwd_wave_lds<SUMMARY>();
     extern __shared__ float lds[];
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
-    float* s_dt = lds + wave * kWave;                   // [channel][step]
+    float* s_bias = lds + wave * kWave;                 // [16], then D [16]
+    float* s_dt = s_bias + 32;                          // [channel][step]
     float* s_ds = s_dt + kInTile;
     float* s_du = s_ds + kInTile;
     float* s_slope = s_du + kInTile;
@@ -92,11 +94,11 @@ __global__ __launch_bounds__(256, 2) void ssm_bwd_kernel(const SsmParams p) {
     int blk, chunk, b0;
     ssm_where(p, blk, chunk, b0);
     if (SUMMARY && chunk == 0) return;                  // nobody ends at the first chunk's summary
-    const int g = blk / p.nblk, c_first = (blk - g * p.nblk) * 64 + wave * 16;
-    const int left = p.Dg - c_first;                    // channels from this wave's first on; <= 0: it only takes part in the barriers
+    const int g = blk / p->nblk, c_first = (blk - g * p->nblk) * 64 + wave * 16;
+    const int left = p->Dg - c_first;                    // channels from this wave's first on; <= 0: it only takes part in the barriers
     if (SUMMARY && left <= 0) return;
-    const int d_first = left > 0 ? g * p.Dg + c_first : 0;
-    const int tile0 = chunk * p.chunk_tiles, tile1 = tile0 + p.chunk_tiles < p.ntile ? tile0 + p.chunk_tiles : p.ntile;
+    const int d_first = left > 0 ? g * p->Dg + c_first : 0;
+    const int tile0 = chunk * p->chunk_tiles, tile1 = tile0 + p->chunk_tiles < p->ntile ? tile0 + p->chunk_tiles : p->ntile;
 
     const int row = lane >> 2, c0 = (lane & 3) * 4, nv = left - c0 < 4 ? left - c0 : 4;
     unsigned cc[4];
@@ -109,45 +111,49 @@ __global__ __launch_bounds__(256, 2) void ssm_bwd_kernel(const SsmParams p) {
     const int ch = lane & 15, q = lane >> 4, dch = d_first + ch;
     const bool has = ch < left;
     auto n0 = [&](int k) { return (k * 4 + q) * RN; };
-    auto count = [&](int k) { const int n = p.N - n0(k); return has ? (n < RN ? n : RN) : 0; };
+    auto count = [&](int k) { const int n = p->N - n0(k); return has ? (n < RN ? n : RN) : 0; };
     unsigned nn[NG][RN];
     float A2[NG][RN], dA[NG][RN];
 #pragma unroll
     for (int k = 0; k < NG; ++k) {
-        const RawVec<float, RN> a = raw_load<float, RN>(p.A + (long long)dch * p.N + n0(k), count(k), p.vec_n);
+        const RawVec<float, RN> a = raw_load<float, RN>(p->A + (long long)dch * p->N + n0(k), count(k), p->vec_n);
 #pragma unroll
         for (int j = 0; j < RN; ++j) {
             A2[k][j] = a.v[j] * kLog2e;
             dA[k][j] = 0.0f;
-            nn[k][j] = n0(k) + j < p.N ? n0(k) + j : (VEC ? 0 : p.N - 1);
+            nn[k][j] = n0(k) + j < p->N ? n0(k) + j : (VEC ? 0 : p->N - 1);
         }
     }
-    const bool clean = left >= 16 && p.N == 4 * RN * NG;
-    const unsigned o_h = (has ? ch : 0) * (unsigned)p.N;
+    if (lane < 32) {
+        const float* src = lane < 16 ? p->dt_bias : p->Dskip;
+        s_bias[lane] = src && has ? src[dch] : 0.0f;
+    }
+    wave_lds_fence();
+    const bool clean = left >= 16 && p->N == 4 * RN * NG;
+    const unsigned o_h = (has ? ch : 0) * (unsigned)p->N;
 
-    for (int b = b0; b < p.B; b += p.b_step) {
+    for (int b = b0; b < p->B; b += p->b_step) {
+        const SsmArgs p = ssm_args();
         const int len = ssm_length(p, b);
-        const T* pu = (const T*)p.u + b * p.u_sb + d_first;
-        const T* pd = (const T*)p.dt + b * p.dt_sb + d_first;
-        const T* pz = p.z ? (const T*)p.z + b * p.z_sb + d_first : nullptr;
-        const T* pg = (const T*)p.dy + b * p.dy_sb + d_first;
-        const T* pB = (const T*)p.Bm + b * p.b_sb + g * p.b_sg;
-        const T* pC = (const T*)p.Cm + b * p.c_sb + g * p.c_sg;
-        const uint8_t* ps = p.starts ? p.starts + b * p.starts_sb : nullptr;
-        const long long obase = (long long)b * p.T * p.D + d_first;           // dense outputs
+        const T* pu = (const T*)p->u + b * p->u_sb + d_first;
+        const T* pd = (const T*)p->dt + b * p->dt_sb + d_first;
+        const T* pz = p->z ? (const T*)p->z + b * p->z_sb + d_first : nullptr;
+        const T* pg = (const T*)p->dy + b * p->dy_sb + d_first;
+        const T* pB = (const T*)p->Bm + b * p->b_sb + g * p->b_sg;
+        const T* pC = (const T*)p->Cm + b * p->c_sb + g * p->c_sg;
+        const uint8_t* ps = p->starts ? p->starts + b * p->starts_sb : nullptr;
+        const long long obase = (long long)b * p->T * p->D + d_first;           // dense outputs
         float gc[NG][RN];                               // what the steps behind add to g of this one
 #pragma unroll
         for (int k = 0; k < NG; ++k) {
-            const RawVec<float, RN> l = raw_load<float, RN>(p.dlast + ((long long)b * p.D + dch) * p.N + n0(k), !SUMMARY && p.dlast ? count(k) : 0, p.vec_n);
+            const RawVec<float, RN> l = raw_load<float, RN>(p->dlast + ((long long)b * p->D + dch) * p->N + n0(k), !SUMMARY && p->dlast ? count(k) : 0, p->vec_n);
 #pragma unroll
             for (int j = 0; j < RN; ++j) gc[k][j] = l.v[j];
-            if (!SUMMARY) {
-                for (int c = p.nchunk - 1; c > chunk; --c) {
-                    const long long at = (((long long)b * p.nchunk + c) * p.D + dch) * p.N + n0(k);
-                    const RawVec<float, RN> P = raw_load<float, RN>(p.sum_p + at, count(k), p.vec_n), S = raw_load<float, RN>(p.sum_s + at, count(k), p.vec_n);
+            if (!SUMMARY && chunk < p->nchunk - 1) {     // from the chunks behind, the last one first
+                const long long at = (((long long)b * p->nchunk + p->nchunk - 1) * p->D + d_first) * p->N;
+                ssm_combine<RN, VEC>(gc[k], p->sum_p + at, p->sum_s + at, -(long long)p->D * p->N, p->nchunk - 1 - chunk, o_h, nn[k]);
 #pragma unroll
-                    for (int j = 0; j < RN; ++j) gc[k][j] = P.v[j] == 0.0f ? S.v[j] : __builtin_fmaf(P.v[j], gc[k][j], S.v[j]);
-                }
+                for (int j = 0; j < RN; ++j) gc[k][j] = j < count(k) ? gc[k][j] : 0.0f;
             }
         }
         float dt_sum = 0.0f;
@@ -158,17 +164,18 @@ __global__ __launch_bounds__(256, 2) void ssm_bwd_kernel(const SsmParams p) {
         RawVec<float, RN> nh[NG];
         unsigned nst = 0;
         auto fetch = [&](int tile) {                    // rows behind the length read the last one
+            const SsmArgs p = ssm_args();
             const long long t0 = (long long)tile * kTile;
             const int last = len - 1 - (int)t0, r = row < last ? row : last, rn = ch < last ? ch : last;
-            if (!SUMMARY) nu = lane_load<T, 4, VEC>(pu + t0 * p.u_st, r * (unsigned)p.u_st, cc);
-            nd = lane_load<T, 4, VEC>(pd + t0 * p.dt_st, r * (unsigned)p.dt_st, cc);
-            if (pz) nz = lane_load<T, 4, VEC>(pz + t0 * p.z_st, r * (unsigned)p.z_st, cc);
-            ng = lane_load<T, 4, VEC>(pg + t0 * p.dy_st, r * (unsigned)p.dy_st, cc);
+            if (!SUMMARY) nu = lane_load<T, 4, VEC>(pu + t0 * p->u_st, r * (unsigned)p->u_st, cc);
+            nd = lane_load<T, 4, VEC>(pd + t0 * p->dt_st, r * (unsigned)p->dt_st, cc);
+            if (pz) nz = lane_load<T, 4, VEC>(pz + t0 * p->z_st, r * (unsigned)p->z_st, cc);
+            ng = lane_load<T, 4, VEC>(pg + t0 * p->dy_st, r * (unsigned)p->dy_st, cc);
 #pragma unroll
             for (int k = 0; k < NG; ++k) {
-                if (!SUMMARY) nB[k] = lane_load<T, RN, VEC>(pB + t0 * p.b_st, rn * (unsigned)p.b_st, nn[k]);
-                nC[k] = lane_load<T, RN, VEC>(pC + t0 * p.c_st, rn * (unsigned)p.c_st, nn[k]);
-                if (!SUMMARY) nh[k] = lane_load<float, RN, VEC>(p.saved + (((long long)b * p.ntile + tile) * p.D + d_first) * p.N, o_h, nn[k]);
+                if (!SUMMARY) nB[k] = lane_load<T, RN, VEC>(pB + t0 * p->b_st, rn * (unsigned)p->b_st, nn[k]);
+                nC[k] = lane_load<T, RN, VEC>(pC + t0 * p->c_st, rn * (unsigned)p->c_st, nn[k]);
+                if (!SUMMARY) nh[k] = lane_load<float, RN, VEC>(p->saved + (((long long)b * p->ntile + tile) * p->D + d_first) * p->N, o_h, nn[k]);
             }
             if (ps) nst = ch <= last ? ps[t0 + rn] : 0;
         };
@@ -176,16 +183,17 @@ __global__ __launch_bounds__(256, 2) void ssm_bwd_kernel(const SsmParams p) {
         if (!SUMMARY) {                                 // steps behind the length: zeros
             const float none[4] = {0.0f, 0.0f, 0.0f, 0.0f};
             for (int tile = tile0 > live ? tile0 : live; tile < tile1; ++tile) {
-                const long long at = obase + (long long)tile * kTile * p.D;
-                const int n = tile * kTile + row < p.T ? nv : 0;
-                const unsigned o = row * (unsigned)p.D + c0;
-                lane_store<T, 4, VEC>((T*)p.du + at, o, none, n);
-                lane_store<T, 4, VEC>((T*)p.ddt + at, o, none, n);
-                if (pz) lane_store<T, 4, VEC>((T*)p.dz + at, o, none, n);
+                const long long at = obase + (long long)tile * kTile * p->D;
+                const int n = tile * kTile + row < p->T ? nv : 0;
+                const unsigned o = row * (unsigned)p->D + c0;
+                lane_store<T, 4, VEC>((T*)p->du + at, o, none, n);
+                lane_store<T, 4, VEC>((T*)p->ddt + at, o, none, n);
+                if (pz) lane_store<T, 4, VEC>((T*)p->dz + at, o, none, n);
             }
         }
         if (tile0 < end) fetch(end - 1);
         for (int tile = end - 1; tile >= tile0; --tile) {
+            const SsmArgs p = ssm_args();
             const int t0 = tile * kTile;
             const bool plain = clean && t0 + kTile <= len, here = t0 + row < len;
             RawVec<T, 4> ru = nu, rz = nz, rg = ng;     // kept as they came: half the registers of a 16-bit type
@@ -210,23 +218,41 @@ __global__ __launch_bounds__(256, 2) void ssm_bwd_kernel(const SsmParams p) {
                 for (int k = 0; k < NG; ++k)
 #pragma unroll
                     for (int j = 0; j < RN; ++j) {
-                        const bool on = t0 + ch < len && n0(k) + j < p.N;
+                        const bool on = t0 + ch < len && n0(k) + j < p->N;
                         Bv[k][j] = on ? Bv[k][j] : 0.0f;
                         Cv[k][j] = on ? Cv[k][j] : 0.0f;
                         h0[k][j] = j < count(k) ? h0[k][j] : 0.0f;
                     }
             }
+            {
+                const f32x4 bias = *(const f32x4*)(s_bias + c0);
+                float dt[4], slope[4], ds[4];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const float raw = (float)nd.v[i] + (i < nv && p.dt_bias ? p.dt_bias[d_first + c0 + i] : 0.0f), gy = (float)rg.v[i];
-                float slope = 1.0f, dt = p.softplus ? softplus_(raw, slope) : raw;
-                if (!plain) dt = here && i < nv ? dt : 0.0f;
-                s_dt[(c0 + i) * kInLd + row] = dt;
-                const float z = pz ? (float)rz.v[i] : 0.0f;
-                s_ds[(c0 + i) * kInLd + row] = pz ? gy * (z * sigmoidf_(z)) : gy;
-                if (!SUMMARY) {
-                    s_du[(c0 + i) * kInLd + row] = dt * (float)ru.v[i];
-                    s_slope[i * 64 + lane] = slope;
+                for (int i = 0; i < 4; ++i) {
+                    dt[i] = (float)nd.v[i] + bias[i];
+                    ds[i] = (float)rg.v[i];
+                    slope[i] = 1.0f;
+                }
+                if (p->softplus) {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) dt[i] = softplus_(dt[i], slope[i]);
+                }
+                if (pz) {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) ds[i] *= (float)rz.v[i] * sigmoidf_((float)rz.v[i]);
+                }
+                if (!plain) {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) dt[i] = here && i < nv ? dt[i] : 0.0f;
+                }
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    s_dt[(c0 + i) * kInLd + row] = dt[i];
+                    s_ds[(c0 + i) * kInLd + row] = ds[i];
+                    if (!SUMMARY) {
+                        s_du[(c0 + i) * kInLd + row] = dt[i] * (float)ru.v[i];
+                        s_slope[i * 64 + lane] = slope[i];
+                    }
                 }
             }
             const unsigned starts = ps ? ssm_start_bits(nst) : 0u;
@@ -265,7 +291,6 @@ __global__ __launch_bounds__(256, 2) void ssm_bwd_kernel(const SsmParams p) {
                             static_for<4>([&](auto ti) {
                                 constexpr int i = decltype(ti)::value, t = tg + i;
                                 const bool fresh = WS && ((starts >> t) & 1u);
-                                float acc = 0.0f;
 #pragma unroll
                                 for (int j = 0; j < RN; ++j) {
                                     const float x = du4[i] * row_bcast<t>(Bv[k][j]), e = __builtin_amdgcn_exp2f(dt4[i] * A2[k][j]);
@@ -273,10 +298,11 @@ __global__ __launch_bounds__(256, 2) void ssm_bwd_kernel(const SsmParams p) {
                                     a[t][j] = fresh ? 0.0f : e;
                                     h[t][j] = fresh ? x : hn;
                                 }
-                                dot_row_bcast<t, RN>(acc, Cv[k], h[t]);
+                                const float acc = dot_row_bcast<t, RN>(Cv[k], h[t]);
                                 s_y[q * kPartLd + t * 16 + ch] = k == 0 ? acc : acc + s_y[q * kPartLd + t * 16 + ch];
                             });
                         });
+                        asm("" : "+v"(Bv[k][0]));       // broadcast anew on the way back: kept, the 16 copies would take 16 registers
                         float hb[4][RN], hc[4][RN];
                         static_for<4>([&](auto gi) {
                             constexpr int tg = 12 - decltype(gi)::value * 4;
@@ -286,9 +312,9 @@ __global__ __launch_bounds__(256, 2) void ssm_bwd_kernel(const SsmParams p) {
                             static_for<4>([&](auto ti) {
                                 constexpr int i = 3 - decltype(ti)::value, t = tg + i;
                                 const bool fresh = WS && ((starts >> t) & 1u);
-                                float gb = 0.0f, aw = 0.0f, vb[RN], vc[RN];
+                                float aw = 0.0f, vb[RN], vc[RN];
                                 fma_row_bcast<t, RN>(gc[k], Cv[k], ds4[i]);          // g_t
-                                dot_row_bcast<t, RN>(gb, Bv[k], gc[k]);
+                                const float gb = dot_row_bcast<t, RN>(Bv[k], gc[k]);
 #pragma unroll
                                 for (int j = 0; j < RN; ++j) {
                                     vb[j] = gc[k][j] * du4[i];
@@ -309,8 +335,13 @@ __global__ __launch_bounds__(256, 2) void ssm_bwd_kernel(const SsmParams p) {
                         });
                         // this wave's sums over its channels, [step][state]: lane (q, ch) has step folded_step(ch), states n0(k) ...
                         float* out = s_bc + wave * (2 * 16 * 4 * RN * NG) + folded_step(ch) * (4 * RN * NG) + n0(k);
+                        if constexpr (RN == 4) {
+                            *(f32x4*)out = f32x4{hb[3][0], hb[3][1], hb[3][2], hb[3][3]};
+                            *(f32x4*)(out + 16 * 4 * RN * NG) = f32x4{hc[3][0], hc[3][1], hc[3][2], hc[3][3]};
+                        } else {
 #pragma unroll
-                        for (int j = 0; j < RN; ++j) { out[j] = hb[3][j]; out[16 * 4 * RN * NG + j] = hc[3][j]; }
+                            for (int j = 0; j < RN; ++j) { out[j] = hb[3][j]; out[16 * 4 * RN * NG + j] = hc[3][j]; }
+                        }
                     });
                 }
             };
@@ -318,6 +349,7 @@ __global__ __launch_bounds__(256, 2) void ssm_bwd_kernel(const SsmParams p) {
             else walk(std::false_type{});
             wave_lds_fence();
             if constexpr (!SUMMARY) {
+                const SsmArgs p = ssm_args();
                 f32x4 gb = *(const f32x4*)(s_gb + row * 16 + c0), aw = *(const f32x4*)(s_aw + row * 16 + c0), ys = *(const f32x4*)(s_y + row * 16 + c0);
 #pragma unroll
                 for (int k = 1; k < 4; ++k) {
@@ -325,29 +357,43 @@ __global__ __launch_bounds__(256, 2) void ssm_bwd_kernel(const SsmParams p) {
                     aw += *(const f32x4*)(s_aw + k * kPartLd + row * 16 + c0);
                     ys += *(const f32x4*)(s_y + k * kPartLd + row * 16 + c0);
                 }
-                float o_u[4], o_dt[4], o_z[4];
+                const f32x4 skip = *(const f32x4*)(s_bias + 16 + c0);
+                float o_u[4], o_dt[4], o_z[4], u[4], gy[4], ds[4];
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    const float u = (float)ru.v[i], z = pz ? (float)rz.v[i] : 0.0f, gy = (float)rg.v[i], dt = s_dt[(c0 + i) * kInLd + row];
-                    const float sig = pz ? sigmoidf_(z) : 0.0f, ds = pz ? gy * (z * sig) : gy;
-                    const float skip = i < nv && p.Dskip ? p.Dskip[d_first + c0 + i] : 0.0f;
-                    o_u[i] = __builtin_fmaf(dt, gb[i], skip * ds);
-                    o_dt[i] = __builtin_fmaf(aw[i], kLn2, u * gb[i]) * s_slope[i * 64 + lane];         // the walk summed A log2(e) w
-                    if (!plain) {
+                    u[i] = (float)ru.v[i];
+                    ds[i] = gy[i] = (float)rg.v[i];
+                }
+                if (pz) {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const float z = (float)rz.v[i], sig = sigmoidf_(z), silu = z * sig;
+                        ds[i] = gy[i] * silu;
+                        o_z[i] = gy[i] * __builtin_fmaf(skip[i], u[i], ys[i]) * __builtin_fmaf(silu, 1.0f - sig, sig);
+                    }
+                }
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    o_u[i] = __builtin_fmaf(s_dt[(c0 + i) * kInLd + row], gb[i], skip[i] * ds[i]);
+                    o_dt[i] = __builtin_fmaf(aw[i], kLn2, u[i] * gb[i]) * s_slope[i * 64 + lane];      // the walk summed A log2(e) w
+                    d_skip[i] = __builtin_fmaf(ds[i], u[i], d_skip[i]);
+                }
+                if (!plain) {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
                         o_u[i] = here ? o_u[i] : 0.0f;
                         o_dt[i] = here ? o_dt[i] : 0.0f;
+                        o_z[i] = here ? o_z[i] : 0.0f;
                     }
-                    o_z[i] = gy * __builtin_fmaf(skip, u, ys[i]) * (sig + z * sig * (1.0f - sig));
-                    if (!plain) o_z[i] = here ? o_z[i] : 0.0f;
-                    d_skip[i] = __builtin_fmaf(ds, u, d_skip[i]);
-                    d_bias[i] += o_dt[i];
                 }
-                const long long to = obase + (long long)t0 * p.D;
-                const unsigned o = row * (unsigned)p.D + c0;
-                const int n = t0 + row < p.T ? nv : 0;
-                lane_store<T, 4, VEC>((T*)p.du + to, o, o_u, n);
-                lane_store<T, 4, VEC>((T*)p.ddt + to, o, o_dt, n);
-                if (pz) lane_store<T, 4, VEC>((T*)p.dz + to, o, o_z, n);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) d_bias[i] += o_dt[i];
+                const long long to = obase + (long long)t0 * p->D;
+                const unsigned o = row * (unsigned)p->D + c0;
+                const int n = t0 + row < p->T ? nv : 0;
+                lane_store<T, 4, VEC>((T*)p->du + to, o, o_u, n);
+                lane_store<T, 4, VEC>((T*)p->ddt + to, o, o_dt, n);
+                if (pz) lane_store<T, 4, VEC>((T*)p->dz + to, o, o_z, n);
                 // dB and dC of the tile over the workgroup's 64 channels
                 __syncthreads();
                 constexpr int W = 4 * RN * NG;          // states as they stand in LDS (N of them exist)
@@ -355,29 +401,30 @@ __global__ __launch_bounds__(256, 2) void ssm_bwd_kernel(const SsmParams p) {
                     const float* src = s_bc + e;
                     const float v = (src[0] + src[2 * 16 * W]) + (src[2 * 2 * 16 * W] + src[3 * 2 * 16 * W]);
                     const int which = e / (16 * W), t = (e / W) % 16, n_ = e % W;
-                    if (n_ < p.N && t0 + t < len) (which ? p.part_c : p.part_b)[(((long long)blk * p.B + b) * p.T + t0 + t) * p.N + n_] = v;
+                    if (n_ < p->N && t0 + t < len) (which ? p->part_c : p->part_b)[(((long long)blk * p->B + b) * p->T + t0 + t) * p->N + n_] = v;
                 }
             }
         }
 #pragma unroll
         for (int k = 0; k < NG; ++k) {
             if (SUMMARY) {
-                const long long at = (((long long)b * p.nchunk + chunk) * p.D + dch) * p.N + n0(k);
+                const long long at = (((long long)b * p->nchunk + chunk) * p->D + dch) * p->N + n0(k);
                 float P[RN];
 #pragma unroll
                 for (int j = 0; j < RN; ++j) P[j] = cut ? 0.0f : __builtin_amdgcn_exp2f(dt_sum * A2[k][j]);
-                raw_store<float, RN>(p.sum_p + at, P, count(k), p.vec_n);
-                raw_store<float, RN>(p.sum_s + at, gc[k], count(k), p.vec_n);
-            } else if (chunk == 0 && p.dstate) {
-                raw_store<float, RN>(p.dstate + ((long long)b * p.D + dch) * p.N + n0(k), gc[k], count(k), p.vec_n);
+                raw_store<float, RN>(p->sum_p + at, P, count(k), p->vec_n);
+                raw_store<float, RN>(p->sum_s + at, gc[k], count(k), p->vec_n);
+            } else if (chunk == 0 && p->dstate) {
+                raw_store<float, RN>(p->dstate + ((long long)b * p->D + dch) * p->N + n0(k), gc[k], count(k), p->vec_n);
             }
         }
     }
     if constexpr (!SUMMARY) {
+        const SsmArgs p = ssm_args();
         // this wave's part of dA, dD, ddt_bias
-        const long long part = (long long)b0 * p.nchunk + chunk;
+        const long long part = (long long)b0 * p->nchunk + chunk;
 #pragma unroll
-        for (int k = 0; k < NG; ++k) raw_store<float, RN>(p.part_a + (part * p.D + dch) * p.N + n0(k), dA[k], count(k), p.vec_n);
+        for (int k = 0; k < NG; ++k) raw_store<float, RN>(p->part_a + (part * p->D + dch) * p->N + n0(k), dA[k], count(k), p->vec_n);
         wave_lds_fence();
 #pragma unroll
         for (int i = 0; i < 4; ++i) { s_dt[(c0 + i) * kInLd + row] = d_skip[i]; s_du[(c0 + i) * kInLd + row] = d_bias[i]; }
@@ -386,8 +433,8 @@ __global__ __launch_bounds__(256, 2) void ssm_bwd_kernel(const SsmParams p) {
             float x = 0.0f, y = 0.0f;
 #pragma unroll
             for (int t = 0; t < kTile; ++t) { x += s_dt[ch * kInLd + t]; y += s_du[ch * kInLd + t]; }
-            p.part_d[part * p.D + dch] = x;
-            p.part_bias[part * p.D + dch] = y;
+            p->part_d[part * p->D + dch] = x;
+            p->part_bias[part * p->D + dch] = y;
         }
     }
 }

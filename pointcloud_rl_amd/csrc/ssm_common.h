@@ -53,27 +53,57 @@ __host__ inline int ssm_rn(int N) { return N <= 4 ? 1 : N <= 8 ? 2 : 4; }      /
 __host__ inline int cdiv(long long a, long long b) { return (int)((a + b - 1) / b); }
 
 #ifdef __HIPCC__
+// The kernel's arguments, read again from the argument segment (scalar loads that hit their cache).  Kept in registers over a tile of a long loop
+// they would not fit: the compiler parks them in lanes of vector registers, and every use costs a vector instruction.
+typedef const __attribute__((address_space(4))) SsmParams* SsmArgs;
+__device__ __forceinline__ SsmArgs ssm_args() {
+    SsmArgs a = (SsmArgs)__builtin_amdgcn_kernarg_segment_ptr();
+    asm volatile("" : "+s"(a));
+    return a;
+}
 // Where this workgroup works: the block index runs channel blocks fastest, then chunks, then batch rows.  Workgroups go to the eight XCDs in
 // turn; when they divide evenly, neighbouring ones -- they read the same B_t and C_t -- are dealt to one XCD.
-__device__ __forceinline__ void ssm_where(const SsmParams& p, int& blk, int& chunk, int& b) {
+__device__ __forceinline__ void ssm_where(SsmArgs p, int& blk, int& chunk, int& b) {
     const unsigned n = gridDim.x;
     unsigned id = blockIdx.x;
     if ((n & 7u) == 0) id = (id & 7u) * (n >> 3) + (id >> 3);
-    const unsigned per = (unsigned)(p.G * p.nblk);
+    const unsigned per = (unsigned)(p->G * p->nblk);
     blk = (int)(id % per);
     const unsigned rest = id / per;
-    chunk = (int)(rest % (unsigned)p.nchunk);
-    b = (int)(rest / (unsigned)p.nchunk);
+    chunk = (int)(rest % (unsigned)p->nchunk);
+    b = (int)(rest / (unsigned)p->nchunk);
 }
-__device__ __forceinline__ int ssm_length(const SsmParams& p, int b) {
-    if (!p.lengths) return p.T;
-    const int n = p.lengths[b];
-    return n < 0 ? 0 : n > p.T ? p.T : n;
+__device__ __forceinline__ int ssm_length(SsmArgs p, int b) {
+    const int* lengths = p->lengths;
+    if (!lengths) return p->T;
+    const int n = lengths[b];
+    return n < 0 ? 0 : n > p->T ? p->T : n;
 }
 // Bit t: step t0 + t begins a new sequence (steps behind the length never do).  Uniform over the wave.
 __device__ __forceinline__ unsigned ssm_start_bits(unsigned char mine) {
     const unsigned long long m = __ballot(mine != 0);
     return (unsigned)__builtin_amdgcn_readfirstlane((int)((unsigned)m & 0xFFFFu));
+}
+// v = P v + S over n chunk summaries, `step` floats apart (the bases are uniform, `off` and `nn` the lane's clamped place).  Four summaries' loads are
+// in flight at a time: the chain is one multiply-add per summary, not one trip to memory.  P == 0: a start (or nothing left) inside the chunk.
+template <int RN, bool VEC>
+__device__ __forceinline__ void ssm_combine(float (&v)[RN], const float* P, const float* S, long long step, int n, unsigned off, const unsigned (&nn)[RN]) {
+    for (int c = 0; c < n; c += 4) {
+        RawVec<float, RN> a[4], s[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const long long at = (c + i < n ? c + i : n - 1) * step;
+            a[i] = lane_load<float, RN, VEC>(P + at, off, nn);
+            s[i] = lane_load<float, RN, VEC>(S + at, off, nn);
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            if (c + i < n) {
+#pragma unroll
+                for (int j = 0; j < RN; ++j) v[j] = a[i].v[j] == 0.0f ? s[i].v[j] : __builtin_fmaf(a[i].v[j], v[j], s[i].v[j]);
+            }
+        }
+    }
 }
 // Orders this wave's LDS writes before its LDS reads (LDS executes a wave's accesses in order: only the compiler has to be told).
 __device__ __forceinline__ void wave_lds_fence() {

@@ -7,7 +7,8 @@ namespace pcrl {
 // SUMMARY: only the states are walked, from zero, and the chunk's summary (product of the decays, end state) is left; otherwise the chunk
 // starts from the combined summaries of the chunks in front of it and y is written.
 template <typename T, int RN, int NG, bool VEC, bool SUMMARY>
-__global__ __launch_bounds__(256) void ssm_fwd_kernel(const SsmParams p) {
+__global__ __launch_bounds__(256) void ssm_fwd_kernel(const SsmParams) {
+    const SsmArgs p = ssm_args();
     constexpr int kWave = 2 * kInTile + (SUMMARY ? 0 : kPartTile);
     __shared__ float lds[4 * kWave];
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
@@ -16,12 +17,12 @@ __global__ __launch_bounds__(256) void ssm_fwd_kernel(const SsmParams p) {
     float* s_y = s_du + kInTile;                        // [state row][step][channel]: sum_n C h
     int blk, chunk, b;
     ssm_where(p, blk, chunk, b);
-    if (SUMMARY && chunk == p.nchunk - 1) return;       // nobody starts from the last chunk's summary
-    const int g = blk / p.nblk, c_first = (blk - g * p.nblk) * 64 + wave * 16;        // first channel of this wave inside its group
-    const int left = p.Dg - c_first;                    // channels from there on
+    if (SUMMARY && chunk == p->nchunk - 1) return;       // nobody starts from the last chunk's summary
+    const int g = blk / p->nblk, c_first = (blk - g * p->nblk) * 64 + wave * 16;        // first channel of this wave inside its group
+    const int left = p->Dg - c_first;                    // channels from there on
     if (left <= 0) return;
-    const int len = ssm_length(p, b), d_first = g * p.Dg + c_first;
-    const int tile0 = chunk * p.chunk_tiles, tile1 = tile0 + p.chunk_tiles < p.ntile ? tile0 + p.chunk_tiles : p.ntile;
+    const int len = ssm_length(p, b), d_first = g * p->Dg + c_first;
+    const int tile0 = chunk * p->chunk_tiles, tile1 = tile0 + p->chunk_tiles < p->ntile ? tile0 + p->chunk_tiles : p->ntile;
 
     // loading layout: step `row` of the tile, channels c0 ... c0 + 3 of the wave (clamped to what exists)
     const int row = lane >> 2, c0 = (lane & 3) * 4, nv = left - c0 < 4 ? left - c0 : 4;
@@ -30,44 +31,42 @@ __global__ __launch_bounds__(256) void ssm_fwd_kernel(const SsmParams p) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         cc[i] = c0 + i < left ? c0 + i : (VEC ? 0 : left - 1);
-        bias[i] = i < nv && p.dt_bias ? p.dt_bias[d_first + c0 + i] : 0.0f;
-        skip[i] = i < nv && p.Dskip ? p.Dskip[d_first + c0 + i] : 0.0f;
+        bias[i] = i < nv && p->dt_bias ? p->dt_bias[d_first + c0 + i] : 0.0f;
+        skip[i] = i < nv && p->Dskip ? p->Dskip[d_first + c0 + i] : 0.0f;
     }
-    const T* pu = (const T*)p.u + b * p.u_sb + d_first;
-    const T* pd = (const T*)p.dt + b * p.dt_sb + d_first;
-    const T* pz = p.z ? (const T*)p.z + b * p.z_sb + d_first : nullptr;
-    T* py = (T*)p.y + (long long)b * p.T * p.D + d_first;
+    const T* pu = (const T*)p->u + b * p->u_sb + d_first;
+    const T* pd = (const T*)p->dt + b * p->dt_sb + d_first;
+    const T* pz = p->z ? (const T*)p->z + b * p->z_sb + d_first : nullptr;
+    T* py = (T*)p->y + (long long)b * p->T * p->D + d_first;
 
     // walking layout: channel ch of the wave, states n0(k) ... n0(k) + RN - 1 of group k
     const int ch = lane & 15, q = lane >> 4, dch = d_first + ch;
     const bool has = ch < left;
     auto n0 = [&](int k) { return (k * 4 + q) * RN; };
-    auto count = [&](int k) { const int n = p.N - n0(k); return has ? (n < RN ? n : RN) : 0; };
+    auto count = [&](int k) { const int n = p->N - n0(k); return has ? (n < RN ? n : RN) : 0; };
     unsigned nn[NG][RN];
     float A2[NG][RN], h[NG][RN];
 #pragma unroll
     for (int k = 0; k < NG; ++k) {
-        const RawVec<float, RN> a = raw_load<float, RN>(p.A + (long long)dch * p.N + n0(k), count(k), p.vec_n);
-        const RawVec<float, RN> s = raw_load<float, RN>(p.state + ((long long)b * p.D + dch) * p.N + n0(k), !SUMMARY && p.state ? count(k) : 0, p.vec_n);
+        const RawVec<float, RN> a = raw_load<float, RN>(p->A + (long long)dch * p->N + n0(k), count(k), p->vec_n);
+        const RawVec<float, RN> s = raw_load<float, RN>(p->state + ((long long)b * p->D + dch) * p->N + n0(k), !SUMMARY && p->state ? count(k) : 0, p->vec_n);
 #pragma unroll
         for (int j = 0; j < RN; ++j) {
             A2[k][j] = a.v[j] * kLog2e;
             h[k][j] = s.v[j];
-            nn[k][j] = n0(k) + j < p.N ? n0(k) + j : (VEC ? 0 : p.N - 1);
+            nn[k][j] = n0(k) + j < p->N ? n0(k) + j : (VEC ? 0 : p->N - 1);
         }
-        if (!SUMMARY) {                                 // h = P h + S over the chunks in front
-            for (int c = 0; c < chunk; ++c) {
-                const long long at = (((long long)b * p.nchunk + c) * p.D + dch) * p.N + n0(k);
-                const RawVec<float, RN> P = raw_load<float, RN>(p.sum_p + at, count(k), p.vec_n), S = raw_load<float, RN>(p.sum_s + at, count(k), p.vec_n);
+        if (!SUMMARY && chunk > 0) {                    // from the chunks in front
+            const long long at = ((long long)b * p->nchunk * p->D + d_first) * p->N;
+            ssm_combine<RN, VEC>(h[k], p->sum_p + at, p->sum_s + at, (long long)p->D * p->N, chunk, (has ? ch : 0) * (unsigned)p->N, nn[k]);
 #pragma unroll
-                for (int j = 0; j < RN; ++j) h[k][j] = P.v[j] == 0.0f ? S.v[j] : __builtin_fmaf(P.v[j], h[k][j], S.v[j]);
-            }
+            for (int j = 0; j < RN; ++j) h[k][j] = j < count(k) ? h[k][j] : 0.0f;
         }
     }
-    const T* pB = (const T*)p.Bm + b * p.b_sb + g * p.b_sg;
-    const T* pC = (const T*)p.Cm + b * p.c_sb + g * p.c_sg;
-    const uint8_t* ps = p.starts ? p.starts + b * p.starts_sb : nullptr;
-    const bool clean = left >= 16 && p.N == 4 * RN * NG;              // every lane's channels and states exist
+    const T* pB = (const T*)p->Bm + b * p->b_sb + g * p->b_sg;
+    const T* pC = (const T*)p->Cm + b * p->c_sb + g * p->c_sg;
+    const uint8_t* ps = p->starts ? p->starts + b * p->starts_sb : nullptr;
+    const bool clean = left >= 16 && p->N == 4 * RN * NG;              // every lane's channels and states exist
     float dt_sum = 0.0f;
     bool cut = false;                                   // a start inside the chunk: nothing from before reaches its end
 
@@ -77,13 +76,13 @@ __global__ __launch_bounds__(256) void ssm_fwd_kernel(const SsmParams p) {
     auto fetch = [&](int tile) {                        // rows behind the length read the last one
         const long long t0 = (long long)tile * kTile;
         const int last = len - 1 - (int)t0, r = row < last ? row : last, rn = ch < last ? ch : last;
-        nu = lane_load<T, 4, VEC>(pu + t0 * p.u_st, r * (unsigned)p.u_st, cc);
-        nd = lane_load<T, 4, VEC>(pd + t0 * p.dt_st, r * (unsigned)p.dt_st, cc);
-        if (!SUMMARY && pz) nz = lane_load<T, 4, VEC>(pz + t0 * p.z_st, r * (unsigned)p.z_st, cc);
+        nu = lane_load<T, 4, VEC>(pu + t0 * p->u_st, r * (unsigned)p->u_st, cc);
+        nd = lane_load<T, 4, VEC>(pd + t0 * p->dt_st, r * (unsigned)p->dt_st, cc);
+        if (!SUMMARY && pz) nz = lane_load<T, 4, VEC>(pz + t0 * p->z_st, r * (unsigned)p->z_st, cc);
 #pragma unroll
         for (int k = 0; k < NG; ++k) {                  // lane r of a 16-lane row: step r
-            nB[k] = lane_load<T, RN, VEC>(pB + t0 * p.b_st, rn * (unsigned)p.b_st, nn[k]);
-            if (!SUMMARY) nC[k] = lane_load<T, RN, VEC>(pC + t0 * p.c_st, rn * (unsigned)p.c_st, nn[k]);
+            nB[k] = lane_load<T, RN, VEC>(pB + t0 * p->b_st, rn * (unsigned)p->b_st, nn[k]);
+            if (!SUMMARY) nC[k] = lane_load<T, RN, VEC>(pC + t0 * p->c_st, rn * (unsigned)p->c_st, nn[k]);
         }
         if (ps) nst = ch <= last ? ps[t0 + rn] : 0;
     };
@@ -97,10 +96,18 @@ __global__ __launch_bounds__(256) void ssm_fwd_kernel(const SsmParams p) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             u[i] = (float)nu.v[i];
-            z[i] = !SUMMARY && pz ? (float)nz.v[i] : 0.0f;
-            float slope;
-            const float raw = (float)nd.v[i] + bias[i];
-            dt[i] = p.softplus ? softplus_(raw, slope) : raw;
+            dt[i] = (float)nd.v[i] + bias[i];
+        }
+        if (p->softplus) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                float slope;
+                dt[i] = softplus_(dt[i], slope);
+            }
+        }
+        if (!SUMMARY && pz) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) z[i] = (float)nz.v[i];
         }
 #pragma unroll
         for (int k = 0; k < NG; ++k)
@@ -116,7 +123,7 @@ __global__ __launch_bounds__(256) void ssm_fwd_kernel(const SsmParams p) {
             for (int k = 0; k < NG; ++k)
 #pragma unroll
                 for (int j = 0; j < RN; ++j) {
-                    const bool on = t0 + ch < len && n0(k) + j < p.N;
+                    const bool on = t0 + ch < len && n0(k) + j < p->N;
                     Bv[k][j] = on ? Bv[k][j] : 0.0f;
                     Cv[k][j] = on ? Cv[k][j] : 0.0f;
                 }
@@ -129,10 +136,10 @@ __global__ __launch_bounds__(256) void ssm_fwd_kernel(const SsmParams p) {
         const unsigned starts = ps ? ssm_start_bits(nst) : 0u;
         wave_lds_fence();
         if (tile + 1 < end) fetch(tile + 1);
-        if (!SUMMARY && p.saved) {
-            float* at = p.saved + (((long long)b * p.ntile + tile) * p.D + d_first) * p.N;
+        if (!SUMMARY && p->saved) {
+            float* at = p->saved + (((long long)b * p->ntile + tile) * p->D + d_first) * p->N;
 #pragma unroll
-            for (int k = 0; k < NG; ++k) lane_store<float, RN, VEC>(at, ch * (unsigned)p.N + n0(k), h[k], count(k));
+            for (int k = 0; k < NG; ++k) lane_store<float, RN, VEC>(at, ch * (unsigned)p->N + n0(k), h[k], count(k));
         }
         auto walk = [&](auto with_starts) {
             static_for<4>([&](auto gi) {
@@ -141,7 +148,7 @@ __global__ __launch_bounds__(256) void ssm_fwd_kernel(const SsmParams p) {
                 static_for<4>([&](auto ti) {
                     constexpr int i = decltype(ti)::value, t = tg + i;
                     const bool fresh = decltype(with_starts)::value && ((starts >> t) & 1u);
-                    float acc = 0.0f;
+                    float acc;
 #pragma unroll
                     for (int k = 0; k < NG; ++k) {
 #pragma unroll
@@ -150,7 +157,7 @@ __global__ __launch_bounds__(256) void ssm_fwd_kernel(const SsmParams p) {
                             const float hn = __builtin_fmaf(__builtin_amdgcn_exp2f(dt4[i] * A2[k][j]), h[k][j], x);
                             h[k][j] = fresh ? x : hn;
                         }
-                        if (!SUMMARY) dot_row_bcast<t, RN>(acc, Cv[k], h[k]);
+                        if (!SUMMARY) acc = k == 0 ? dot_row_bcast<t, RN>(Cv[k], h[k]) : acc + dot_row_bcast<t, RN>(Cv[k], h[k]);
                     }
                     if (SUMMARY) dt_sum += dt4[i];
                     else s_y[q * kPartLd + t * 16 + ch] = acc;
@@ -166,30 +173,34 @@ __global__ __launch_bounds__(256) void ssm_fwd_kernel(const SsmParams p) {
             for (int k = 1; k < 4; ++k) s += *(const f32x4*)(s_y + k * kPartLd + row * 16 + c0);
             float out[4];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                out[i] = __builtin_fmaf(skip[i], u[i], s[i]);
-                if (pz) out[i] *= z[i] * sigmoidf_(z[i]);
-                if (!plain) out[i] = here ? out[i] : 0.0f;
+            for (int i = 0; i < 4; ++i) out[i] = __builtin_fmaf(skip[i], u[i], s[i]);
+            if (pz) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) out[i] *= z[i] * sigmoidf_(z[i]);
             }
-            lane_store<T, 4, VEC>(py + (long long)t0 * p.D, row * (unsigned)p.D + c0, out, t0 + row < p.T ? nv : 0);
+            if (!plain) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) out[i] = here ? out[i] : 0.0f;
+            }
+            lane_store<T, 4, VEC>(py + (long long)t0 * p->D, row * (unsigned)p->D + c0, out, t0 + row < p->T ? nv : 0);
         }
     }
     if (!SUMMARY) {                                     // steps behind the length: zeros
         const float none[4] = {0.0f, 0.0f, 0.0f, 0.0f};
         for (int tile = tile0 > live ? tile0 : live; tile < tile1; ++tile)
-            lane_store<T, 4, VEC>(py + (long long)tile * kTile * p.D, row * (unsigned)p.D + c0, none, tile * kTile + row < p.T ? nv : 0);
+            lane_store<T, 4, VEC>(py + (long long)tile * kTile * p->D, row * (unsigned)p->D + c0, none, tile * kTile + row < p->T ? nv : 0);
     }
 #pragma unroll
     for (int k = 0; k < NG; ++k) {
         if (SUMMARY) {
-            const long long at = (((long long)b * p.nchunk + chunk) * p.D + dch) * p.N + n0(k);
+            const long long at = (((long long)b * p->nchunk + chunk) * p->D + dch) * p->N + n0(k);
             float P[RN];
 #pragma unroll
             for (int j = 0; j < RN; ++j) P[j] = cut ? 0.0f : __builtin_amdgcn_exp2f(dt_sum * A2[k][j]);
-            raw_store<float, RN>(p.sum_p + at, P, count(k), p.vec_n);
-            raw_store<float, RN>(p.sum_s + at, h[k], count(k), p.vec_n);
-        } else if (p.last && chunk == p.nchunk - 1) {
-            raw_store<float, RN>(p.last + ((long long)b * p.D + dch) * p.N + n0(k), h[k], count(k), p.vec_n);
+            raw_store<float, RN>(p->sum_p + at, P, count(k), p->vec_n);
+            raw_store<float, RN>(p->sum_s + at, h[k], count(k), p->vec_n);
+        } else if (p->last && chunk == p->nchunk - 1) {
+            raw_store<float, RN>(p->last + ((long long)b * p->D + dch) * p->N + n0(k), h[k], count(k), p->vec_n);
         }
     }
 }
@@ -291,11 +302,11 @@ SsmPlan ssm_plan(const pcrl_ssm_desc* d, bool backward) {
     const int ntile = cdiv(d->T, kTile);
     plan.nblk = cdiv(d->D / d->G, 64);
     const long long blocks = (long long)d->B * d->G * plan.nblk;
-    long long chunks = 4LL * num_cus() / blocks;
+    const long long cus = num_cus();
+    long long chunks = 2 * blocks >= 3 * cus ? 1 : ((backward ? 2 : 4) * cus + blocks - 1) / blocks;
     const char* e = getenv(backward ? "PCRL_X_BCHUNKS" : "PCRL_X_CHUNKS");
     if (e) chunks = atoi(e);
-    if (chunks > ntile / 2) chunks = ntile / 2;
-    if (chunks < 2) chunks = 1;
+    if (chunks > ntile) chunks = ntile;
     plan.chunk_tiles = cdiv(ntile, chunks);
     plan.nchunk = cdiv(ntile, plan.chunk_tiles);
     return plan;
