@@ -30,9 +30,12 @@ __global__ __launch_bounds__(256) void dropout_kernel(const DropoutParams p) {
     } else {
         x = raw_zero<T, 8>(), res = raw_zero<T, 8>();
         long long row = e0 / p.cols, col = e0 - row * p.cols;
-        for (int k = 0; k < left; ++k) {
-            x.v[k] = px[row * p.x_ld + col];
-            if (pr) res.v[k] = pr[row * p.residual_ld + col];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+            if (k < left) {
+                x.v[k] = px[row * p.x_ld + col];
+                if (pr) res.v[k] = pr[row * p.residual_ld + col];
+            }
             if (++col == p.cols) { col = 0; ++row; }
         }
     }

@@ -5,8 +5,11 @@
 
 namespace pcrl {
 
+constexpr int kConvV = 4;                              // adjacent channels of a thread
+constexpr int kRun = 8;                                // steps a forward thread takes
+
 struct ConvParams {
-    int B, T, D, silu, vec, nrun, run;                 // runs of `run` steps
+    int B, T, D, silu, vec, vec_w, nrun, run;          // vec, vec_w: whole vectors of the activations, of the weights; runs of `run` steps (backward)
     long long x_sb, x_st, dy_sb, dy_st, starts_sb;
     const void *x, *state, *dy, *dlast;
     const float *weight, *bias;
@@ -51,6 +54,32 @@ __device__ __forceinline__ void conv_window(const ConvParams& p, int b, int d0, 
     }
 }
 
+// The W taps of the thread's channels: V W adjacent floats.
+template <int V, int W>
+__device__ __forceinline__ void conv_weights(const ConvParams& p, int d0, int nv, float (&w)[W][V], float (&bias)[V]) {
+    if (p.vec_w && nv == V) {
+        const f32x4* src = (const f32x4*)(p.weight + (long long)d0 * W);
+        float flat[V * W];
+#pragma unroll
+        for (int e = 0; e < V * W / 4; ++e) {
+            const f32x4 x = src[e];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) flat[4 * e + i] = x[i];
+        }
+#pragma unroll
+        for (int i = 0; i < V; ++i)
+#pragma unroll
+            for (int k = 0; k < W; ++k) w[k][i] = flat[i * W + k];
+    } else {
+#pragma unroll
+        for (int i = 0; i < V; ++i)
+#pragma unroll
+            for (int k = 0; k < W; ++k) w[k][i] = i < nv ? p.weight[(long long)(d0 + i) * W + k] : 0.0f;
+    }
+#pragma unroll
+    for (int i = 0; i < V; ++i) bias[i] = i < nv && p.bias ? p.bias[d0 + i] : 0.0f;
+}
+
 template <typename T, int V, int W>
 __global__ __launch_bounds__(256) void conv_fwd_kernel(const ConvParams p) {
     const int nvec = (p.D + V - 1) / V;
@@ -68,48 +97,61 @@ __global__ __launch_bounds__(256) void conv_fwd_kernel(const ConvParams p) {
         return;
     }
     float w[W][V], bias[V];
-#pragma unroll
-    for (int i = 0; i < V; ++i) {
-        bias[i] = i < nv && p.bias ? p.bias[d0 + i] : 0.0f;
-#pragma unroll
-        for (int k = 0; k < W; ++k) w[k][i] = i < nv ? p.weight[(long long)(d0 + i) * W + k] : 0.0f;
-    }
-    const int t_first = q * p.run, t_last = t_first + p.run < p.T ? t_first + p.run : p.T;
-    if (t_first < len) conv_window<T, V, W>(p, b, d0, nv, t_first, win);
+    conv_weights<V, W>(p, d0, nv, w, bias);
+    const int t_first = q * kRun, t_last = t_first + kRun < p.T ? t_first + kRun : p.T;
     const T* px = (const T*)p.x + b * p.x_sb + d0;
     T* py = (T*)p.y + (long long)b * p.T * p.D + d0;
-    constexpr int U = 4;                               // rows in flight
-    for (int t0 = t_first; t0 < t_last; t0 += U) {
-        RawVec<T, V> raw[U];
-        bool st[U];
+    RawVec<T, V> raw[kRun];                            // the whole run in flight, the window's rows with it
+    bool st[kRun];
+    // Almost every wave: all rows exist and no start is near (one test for the wave, then nothing but loads).
+    const bool easy = p.vec && !p.starts && t_first >= W - 1 && t_first + kRun <= len;
+    if (__all(easy)) {
+        RawVec<T, V> before[W];
 #pragma unroll
-        for (int k = 0; k < U; ++k) {
-            const int t = t0 + k;
+        for (int k = 0; k < W - 1; ++k) before[k] = raw_load<T, V>(px + (long long)(t_first - (W - 1) + k) * p.x_st, V, true);
+#pragma unroll
+        for (int k = 0; k < kRun; ++k) {
+            raw[k] = raw_load<T, V>(px + (long long)(t_first + k) * p.x_st, V, true);
+            st[k] = false;
+        }
+#pragma unroll
+        for (int k = 0; k < W - 1; ++k)
+#pragma unroll
+            for (int i = 0; i < V; ++i) win[k][i] = (float)before[k].v[i];
+    } else {
+#pragma unroll
+        for (int k = 0; k < kRun; ++k) {
+            const int t = t_first + k;
             const bool on = t < t_last && t < len;
             raw[k] = raw_load<T, V>(px + (long long)t * p.x_st, on ? nv : 0, p.vec);
             st[k] = p.starts && on && p.starts[b * p.starts_sb + t];
         }
+        conv_window<T, V, W>(p, b, d0, t_first < len ? nv : 0, t_first, win);
+    }
 #pragma unroll
-        for (int k = 0; k < U; ++k) {
-            const int t = t0 + k;
-            if (t >= t_last) break;
-            float out[V];
+    for (int k = 0; k < kRun; ++k) {
+        const int t = t_first + k;
+        float out[V];
 #pragma unroll
-            for (int i = 0; i < V; ++i) {
-                if (st[k])
+        for (int i = 0; i < V; ++i) {
+            if (st[k])
 #pragma unroll
-                    for (int j = 0; j < W - 1; ++j) win[j][i] = 0.0f;
-                win[W - 1][i] = (float)raw[k].v[i];
-                float acc = bias[i];
+                for (int j = 0; j < W - 1; ++j) win[j][i] = 0.0f;
+            win[W - 1][i] = (float)raw[k].v[i];
+            float acc = bias[i];
 #pragma unroll
-                for (int j = 0; j < W; ++j) acc = __builtin_fmaf(w[j][i], win[j][i], acc);
-                if (p.silu) acc *= sigmoidf_(acc);
-                out[i] = t < len ? acc : 0.0f;
+            for (int j = 0; j < W; ++j) acc = __builtin_fmaf(w[j][i], win[j][i], acc);
+            out[i] = acc;
 #pragma unroll
-                for (int j = 0; j < W - 1; ++j) win[j][i] = win[j + 1][i];
-            }
-            raw_store<T, V>(py + (long long)t * p.D, out, nv, p.vec);
+            for (int j = 0; j < W - 1; ++j) win[j][i] = win[j + 1][i];
         }
+        if (p.silu) {
+#pragma unroll
+            for (int i = 0; i < V; ++i) out[i] *= sigmoidf_(out[i]);
+        }
+#pragma unroll
+        for (int i = 0; i < V; ++i) out[i] = t < len ? out[i] : 0.0f;
+        raw_store<T, V>(py + (long long)t * p.D, out, t < t_last ? nv : 0, p.vec);
     }
 }
 
@@ -153,15 +195,15 @@ template <typename T, int V, int W>
 __global__ __launch_bounds__(256) void conv_bwd_kernel(const ConvParams p) {
     extern __shared__ float s_part[];                  // [4][W + 1][64 V]
     // a workgroup: 64 channel vectors x 4 walkers; walker (blockIdx.y, k) takes every parts-th (b, run)
-    const int lane = threadIdx.x & 63, k4 = threadIdx.x >> 6;
+    const int lane = threadIdx.x & 63, k4 = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int d0 = (blockIdx.x * 64 + lane) * V, nv = p.D - d0 < V ? p.D - d0 : V;       // nv <= 0: no channel
     float w[W][V], bias[V], dw[W][V], db[V];
+    conv_weights<V, W>(p, d0, nv, w, bias);
 #pragma unroll
     for (int i = 0; i < V; ++i) {
-        bias[i] = i < nv && p.bias ? p.bias[d0 + i] : 0.0f;
         db[i] = 0.0f;
 #pragma unroll
-        for (int k = 0; k < W; ++k) { w[k][i] = i < nv ? p.weight[(long long)(d0 + i) * W + k] : 0.0f; dw[k][i] = 0.0f; }
+        for (int k = 0; k < W; ++k) dw[k][i] = 0.0f;
     }
     const long long lines = (long long)p.B * p.nrun;
     for (long long line = (long long)blockIdx.y * 4 + k4; line < lines; line += 4LL * p.parts) {
@@ -192,12 +234,21 @@ __global__ __launch_bounds__(256) void conv_bwd_kernel(const ConvParams p) {
         for (int s0 = t_first; s0 < stop; s0 += U) {
             RawVec<T, V> rx[U], rg[U];
             bool st[U];
+            if (p.vec && !ps && s0 + U <= stop) {      // (uniform over the wave)
 #pragma unroll
-            for (int k = 0; k < U; ++k) {
-                const bool on = s0 + k < stop;
-                rx[k] = raw_load<T, V>(px + (long long)(s0 + k) * p.x_st, on ? nv : 0, p.vec);
-                rg[k] = raw_load<T, V>(pg + (long long)(s0 + k) * p.dy_st, on ? nv : 0, p.vec);
-                st[k] = ps && on && ps[s0 + k];
+                for (int k = 0; k < U; ++k) {
+                    rx[k] = raw_load<T, V>(px + (long long)(s0 + k) * p.x_st, nv, true);
+                    rg[k] = raw_load<T, V>(pg + (long long)(s0 + k) * p.dy_st, nv, true);
+                    st[k] = false;
+                }
+            } else {
+#pragma unroll
+                for (int k = 0; k < U; ++k) {
+                    const bool on = s0 + k < stop;
+                    rx[k] = raw_load<T, V>(px + (long long)(s0 + k) * p.x_st, on ? nv : 0, p.vec);
+                    rg[k] = raw_load<T, V>(pg + (long long)(s0 + k) * p.dy_st, on ? nv : 0, p.vec);
+                    st[k] = ps && on && ps[s0 + k];
+                }
             }
 #pragma unroll
             for (int k = 0; k < U; ++k) {
@@ -310,6 +361,7 @@ static void conv_fill(ConvParams& p, const pcrl_conv_desc* d) {
     p.B = d->B, p.T = d->T, p.D = d->D, p.silu = d->silu != 0;
     p.x = d->x, p.x_sb = d->x_sb, p.x_st = d->x_st, p.weight = d->weight, p.bias = d->bias, p.state = d->state;
     p.starts = d->starts, p.starts_sb = d->starts_sb, p.lengths = d->lengths;
+    p.vec_w = (uintptr_t)d->weight % 16 == 0;
 }
 static bool conv_vec(const pcrl_conv_desc* d, int V, const void* const* extra, int n) {
     const size_t bytes = (size_t)V * elem_bytes(d->dtype);
@@ -328,9 +380,7 @@ static int conv_fwd(ConvParams& p, hipStream_t s) {
         PCRL_CHECK_LAUNCH("conv_step_kernel");
         return PCRL_OK;
     }
-    p.run = 16;
-    while (p.run > 4 && nvec * p.B * ((p.T + p.run - 1) / p.run) < 256LL * num_cus()) p.run >>= 1;
-    p.nrun = (p.T + p.run - 1) / p.run;
+    p.nrun = (p.T + kRun - 1) / kRun;
     const long long blocks = (nvec * p.B * (p.nrun + 1) + 255) / 256;
     if (blocks > 0x7FFFFFFFLL) return fail(PCRL_E_ARG, "pcrl_short_conv_fwd: too many workgroups");
     conv_fwd_kernel<T, V, W><<<dim3((unsigned)blocks), 256, 0, s>>>(p);
@@ -338,12 +388,12 @@ static int conv_fwd(ConvParams& p, hipStream_t s) {
     return PCRL_OK;
 }
 static void conv_bwd_plan(const pcrl_conv_desc* d, int& run, int& nrun, int& parts) {
-    const int V = 16 / elem_bytes(d->dtype);
+    const int V = kConvV;
     const long long cols = (d->D + 64 * V - 1) / (64 * V);
     run = 32;
-    while (run > 8 && cols * d->B * ((d->T + run - 1) / run) < 8LL * num_cus()) run >>= 1;
+    while (run > 8 && cols * d->B * ((d->T + run - 1) / run) < 16LL * num_cus()) run >>= 1;
     nrun = (d->T + run - 1) / run;
-    const long long lines = (long long)d->B * nrun, want = 2LL * num_cus() / cols;
+    const long long lines = (long long)d->B * nrun, want = 4LL * num_cus() / cols;
     long long n = (lines + 3) / 4;
     if (n > want) n = want;
     parts = n < 1 ? 1 : (int)n;
@@ -379,12 +429,12 @@ extern "C" int pcrl_short_conv_fwd(const pcrl_conv_desc* d, void* y, void* last_
     conv_fill(p, d);
     p.y = y, p.last = last_state;
     const void* extra[2] = {y, last_state};
-    p.vec = conv_vec(d, 16 / elem_bytes(d->dtype), extra, 2);
+    p.vec = conv_vec(d, kConvV, extra, 2);
     hipStream_t s = (hipStream_t)stream;
 #define PCRL_CONV_ARGS (p, s)
-    if (d->dtype == PCRL_DT_F32) { PCRL_CONV_W(conv_fwd, float, 4) }
-    if (d->dtype == PCRL_DT_BF16) { PCRL_CONV_W(conv_fwd, __bf16, 8) }
-    PCRL_CONV_W(conv_fwd, _Float16, 8)
+    if (d->dtype == PCRL_DT_F32) { PCRL_CONV_W(conv_fwd, float, kConvV) }
+    if (d->dtype == PCRL_DT_BF16) { PCRL_CONV_W(conv_fwd, __bf16, kConvV) }
+    PCRL_CONV_W(conv_fwd, _Float16, kConvV)
 #undef PCRL_CONV_ARGS
 }
 
@@ -407,13 +457,13 @@ extern "C" int pcrl_short_conv_bwd(const pcrl_conv_desc* d, const void* dy, int6
     conv_fill(p, d);
     conv_bwd_plan(d, p.run, p.nrun, p.parts);
     p.dy = dy, p.dy_sb = dy_sb, p.dy_st = dy_st, p.dlast = dlast, p.dx = dx, p.dstate = dstate, p.part = (float*)workspace;
-    const int V = 16 / elem_bytes(d->dtype);
+    const int V = kConvV;
     const void* extra[4] = {dy, dlast, dx, dstate};
     p.vec = conv_vec(d, V, extra, 4) && dy_sb % V == 0 && dy_st % V == 0;
     hipStream_t s = (hipStream_t)stream;
 #define PCRL_CONV_ARGS (p, dweight, dbias, s)
-    if (d->dtype == PCRL_DT_F32) { PCRL_CONV_W(conv_bwd, float, 4) }
-    if (d->dtype == PCRL_DT_BF16) { PCRL_CONV_W(conv_bwd, __bf16, 8) }
-    PCRL_CONV_W(conv_bwd, _Float16, 8)
+    if (d->dtype == PCRL_DT_F32) { PCRL_CONV_W(conv_bwd, float, kConvV) }
+    if (d->dtype == PCRL_DT_BF16) { PCRL_CONV_W(conv_bwd, __bf16, kConvV) }
+    PCRL_CONV_W(conv_bwd, _Float16, kConvV)
 #undef PCRL_CONV_ARGS
 }

@@ -206,48 +206,66 @@ __global__ __launch_bounds__(256) void ssm_fwd_kernel(const SsmParams) {
 }
 
 // One step.  The state is 8 N bytes per channel of traffic against a few of everything else, so lanes run along it: LPC lanes per channel, four
-// states each (16-byte accesses when N % 4 == 0), the sum over the states inside the group of LPC lanes.
+// states each (16-byte accesses when N % 4 == 0), the sum over the states inside the group of LPC lanes.  A workgroup keeps its A and walks
+// batch rows b, b + b_step, ..., the next row's loads in flight while this one is computed.
 struct SsmStepParams {
     SsmParams s;
     float* state_out;
-    int lpc;                           // lanes per channel: 1, 2, 4 or 8
-    int vec4;                          // N % 4 == 0 and A and the states aligned: whole 16-byte accesses
+    int rows;                          // batch rows a workgroup holds at once (more than 1 when D is small)
+    int b_step;
 };
-template <typename T>
+template <typename T, int LPC, bool VEC>
 __global__ __launch_bounds__(256) void ssm_step_kernel(const SsmStepParams q) {
     const SsmParams& p = q.s;
-    const long long idx = (long long)blockIdx.x * 256 + threadIdx.x;
-    const long long pair = idx / q.lpc;
-    const int k = (int)(idx - pair * q.lpc) * 4;
-    const bool on = pair < (long long)p.B * p.D;
-    const int b = on ? (int)(pair / p.D) : 0, d = on ? (int)(pair - (long long)b * p.D) : 0, g = d / p.Dg;
-    const int n = on ? (p.N - k < 4 ? p.N - k : 4) : 0;
-    const bool vec = q.vec4;
-    const float u = on ? (float)((const T*)p.u)[b * p.u_sb + d] : 0.0f;
-    float dt = on ? (float)((const T*)p.dt)[b * p.dt_sb + d] + (p.dt_bias ? p.dt_bias[d] : 0.0f) : 0.0f, slope;
-    if (p.softplus) dt = softplus_(dt, slope);
-    const bool fresh = on && p.starts && p.starts[b * p.starts_sb];
-    const RawVec<float, 4> h = raw_load<float, 4>(p.state + pair * p.N + k, fresh ? 0 : n, vec);
-    const RawVec<float, 4> A = raw_load<float, 4>(p.A + (long long)d * p.N + k, n, vec);
-    const RawVec<T, 4> Bv = raw_load<T, 4>((const T*)p.Bm + b * p.b_sb + g * p.b_sg + k, n, false);
-    const RawVec<T, 4> Cv = raw_load<T, 4>((const T*)p.Cm + b * p.c_sb + g * p.c_sg + k, n, false);
-    const float du = dt * u;
-    float out[4], acc = 0.0f;
+    const unsigned width = (unsigned)p.D * LPC, flat = blockIdx.x * 256 + threadIdx.x;       // lanes of one batch row
+    const unsigned r = q.rows > 1 ? threadIdx.x / width : 0, w = q.rows > 1 ? threadIdx.x - r * width : flat;
+    const bool lane_on = q.rows > 1 ? r < (unsigned)q.rows : flat < width;
+    const int d = lane_on ? (int)(w / LPC) : 0, k = (int)(w % LPC) * 4, g = d / p.Dg;
+    const int n = lane_on ? (p.N - k < 4 ? p.N - k : 4) : 0;
+    float A2[4];
+    {
+        const RawVec<float, 4> A = raw_load<float, 4>(p.A + (long long)d * p.N + k, n, VEC);
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-        const float x = du * (float)Bv.v[j];
-        out[j] = fresh ? x : __builtin_fmaf(__builtin_amdgcn_exp2f(dt * (A.v[j] * kLog2e)), h.v[j], x);
-        acc = j < n ? __builtin_fmaf((float)Cv.v[j], out[j], acc) : acc;
+        for (int j = 0; j < 4; ++j) A2[j] = A.v[j] * kLog2e;
     }
-    raw_store<float, 4>(q.state_out + pair * p.N + k, out, n, vec);
-    for (int off = q.lpc >> 1; off > 0; off >>= 1) acc += __shfl_xor(acc, off, 64);
-    if (on && k == 0) {
-        if (p.Dskip) acc = __builtin_fmaf(p.Dskip[d], u, acc);
-        if (p.z) {
-            const float z = (float)((const T*)p.z)[b * p.z_sb + d];
-            acc *= z * sigmoidf_(z);
+    const float bias = lane_on && p.dt_bias ? p.dt_bias[d] : 0.0f, skip = lane_on && p.Dskip ? p.Dskip[d] : 0.0f;
+    struct Row { T u, dt, z; RawVec<T, 4> B, C; RawVec<float, 4> h; bool fresh; } cur, next;
+    auto load = [&](Row& x, int b) {
+        const bool on = lane_on && b < p.B;
+        x.u = on ? ((const T*)p.u)[b * p.u_sb + d] : (T)0.0f;
+        x.dt = on ? ((const T*)p.dt)[b * p.dt_sb + d] : (T)0.0f;
+        x.z = on && p.z ? ((const T*)p.z)[b * p.z_sb + d] : (T)0.0f;
+        x.fresh = on && p.starts && p.starts[b * p.starts_sb];
+        x.B = raw_load<T, 4>((const T*)p.Bm + b * p.b_sb + g * p.b_sg + k, on ? n : 0, VEC);
+        x.C = raw_load<T, 4>((const T*)p.Cm + b * p.c_sb + g * p.c_sg + k, on ? n : 0, VEC);
+        x.h = raw_load<float, 4>(p.state + ((long long)b * p.D + d) * p.N + k, on ? n : 0, VEC);
+    };
+    int b = blockIdx.y * q.rows + (int)r;
+    const int first = blockIdx.y * q.rows;
+    load(cur, b);
+    for (int b0 = first; b0 < p.B; b0 += q.b_step, b += q.b_step) {
+        if (b0 + q.b_step < p.B) load(next, b + q.b_step);
+        const float u = (float)cur.u;
+        float dt = (float)cur.dt + bias, slope;
+        if (p.softplus) dt = softplus_(dt, slope);
+        const float du = dt * u;
+        float out[4], acc = 0.0f;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const float x = du * (float)cur.B.v[j], hn = __builtin_fmaf(__builtin_amdgcn_exp2f(dt * A2[j]), cur.h.v[j], x);
+            out[j] = cur.fresh ? x : hn;
+            acc = j < n ? __builtin_fmaf((float)cur.C.v[j], out[j], acc) : acc;
         }
-        ((T*)p.y)[pair] = (T)acc;
+        const bool on = lane_on && b < p.B;
+        raw_store<float, 4>(q.state_out + ((long long)b * p.D + d) * p.N + k, out, on ? n : 0, VEC);
+#pragma unroll
+        for (int off = LPC >> 1; off > 0; off >>= 1) acc += __shfl_xor(acc, off, 64);
+        if (on && k == 0) {
+            acc = __builtin_fmaf(skip, u, acc);
+            if (p.z) acc *= (float)cur.z * sigmoidf_((float)cur.z);
+            ((T*)p.y)[(long long)b * p.D + d] = (T)acc;
+        }
+        cur = next;
     }
 }
 
@@ -330,6 +348,19 @@ static int launch_fwd_n(const SsmParams& p, hipStream_t s) {
 template <typename T>
 static int launch_fwd_t(const SsmParams& p, bool vec, hipStream_t s) { return vec ? launch_fwd_n<T, true>(p, s) : launch_fwd_n<T, false>(p, s); }
 
+template <typename T, int LPC>
+static void launch_step_n(const SsmStepParams& q, bool vec, dim3 grid, hipStream_t s) {
+    if (vec) ssm_step_kernel<T, LPC, true><<<grid, 256, 0, s>>>(q);
+    else ssm_step_kernel<T, LPC, false><<<grid, 256, 0, s>>>(q);
+}
+template <typename T>
+static void launch_step(const SsmStepParams& q, int lpc, bool vec, dim3 grid, hipStream_t s) {
+    if (lpc == 1) launch_step_n<T, 1>(q, vec, grid, s);
+    else if (lpc == 2) launch_step_n<T, 2>(q, vec, grid, s);
+    else if (lpc == 4) launch_step_n<T, 4>(q, vec, grid, s);
+    else launch_step_n<T, 8>(q, vec, grid, s);
+}
+
 static size_t fwd_summary(const pcrl_ssm_desc* d, const SsmPlan& plan) {                 // floats, a multiple of 16 bytes
     return plan.nchunk > 1 ? ((size_t)d->B * plan.nchunk * d->N * d->D + 3) & ~(size_t)3 : 0;
 }
@@ -376,15 +407,23 @@ extern "C" int pcrl_ssm_step(const pcrl_ssm_desc* d, void* y, float* state_out, 
     SsmStepParams q;
     ssm_fill(q.s, d);
     q.s.y = y, q.state_out = state_out;
-    q.vec4 = (d->N & 3) == 0 && ((uintptr_t)d->state | (uintptr_t)state_out | (uintptr_t)d->A) % 16 == 0;
-    q.lpc = d->N <= 4 ? 1 : d->N <= 8 ? 2 : d->N <= 16 ? 4 : 8;
-    const long long threads = (long long)d->B * d->D * q.lpc;
-    if ((threads + 255) / 256 > 0x7FFFFFFFLL) return fail(PCRL_E_ARG, "pcrl_ssm_step: too many workgroups");
-    const dim3 grid((unsigned)((threads + 255) / 256));
+    const int lpc = d->N <= 4 ? 1 : d->N <= 8 ? 2 : d->N <= 16 ? 4 : 8;
+    const bool vec = (d->N & 3) == 0 && ((uintptr_t)d->state | (uintptr_t)state_out | (uintptr_t)d->A) % 16 == 0 &&
+                     ((uintptr_t)d->Bm | (uintptr_t)d->Cm) % (4 * (uintptr_t)elem_bytes(d->dtype)) == 0 && (d->b_sb | d->b_sg | d->c_sb | d->c_sg) % 4 == 0;
+    const long long width = (long long)d->D * lpc;
+    if (width > 0x7FFFFFFFLL) return fail(PCRL_E_ARG, "pcrl_ssm_step: D = %d", d->D);
+    q.rows = width < 256 ? (int)(256 / width) : 1;
+    const unsigned gx = q.rows > 1 ? 1u : (unsigned)cdiv(width, 256), groups = (unsigned)cdiv(d->B, q.rows);
+    // workgroups for every row, up to about eight per CU; beyond that each walks several rows
+    unsigned gy = (unsigned)((8LL * num_cus() + gx - 1) / gx);
+    gy = gy < 1 ? 1 : gy > 65535 ? 65535 : gy;
+    gy = gy < groups ? gy : groups;
+    q.b_step = (int)gy * q.rows;
+    const dim3 grid(gx, gy);
     hipStream_t s = (hipStream_t)stream;
-    if (d->dtype == PCRL_DT_F32) ssm_step_kernel<float><<<grid, 256, 0, s>>>(q);
-    else if (d->dtype == PCRL_DT_BF16) ssm_step_kernel<__bf16><<<grid, 256, 0, s>>>(q);
-    else ssm_step_kernel<_Float16><<<grid, 256, 0, s>>>(q);
+    if (d->dtype == PCRL_DT_F32) launch_step<float>(q, lpc, vec, grid, s);
+    else if (d->dtype == PCRL_DT_BF16) launch_step<__bf16>(q, lpc, vec, grid, s);
+    else launch_step<_Float16>(q, lpc, vec, grid, s);
     PCRL_CHECK_LAUNCH("ssm_step_kernel");
     return PCRL_OK;
 }
