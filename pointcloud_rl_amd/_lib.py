@@ -116,6 +116,19 @@ class SsmGrads(ctypes.Structure):
     _fields_ = [(k, ctypes.c_void_p) for k in ("du", "ddt", "dz", "dB", "dC", "dA", "dD", "ddt_bias", "dstate")]
 
 
+_P, _I, _L, _Z, _U = ctypes.c_void_p, ctypes.c_int32, ctypes.c_int64, ctypes.c_size_t, ctypes.c_uint64
+_SEQUENCE_ARGTYPES = {
+    "pcrl_short_conv_fwd": [_P, _P, _P, _P],
+    "pcrl_short_conv_bwd_workspace_bytes": [_P, _P],
+    "pcrl_short_conv_bwd": [_P, _P, _L, _L, _P, _P, _P, _P, _P, _P, _Z, _P],
+    "pcrl_ssm_scan_bytes": [_P, _P, _P, _P],
+    "pcrl_ssm_scan_fwd": [_P, _P, _P, _P, _P, _Z, _P],
+    "pcrl_ssm_scan_bwd": [_P, _P, _P, _L, _L, _P, _P, _P, _Z, _P],
+    "pcrl_ssm_step": [_P, _P, _P, _P],
+    "pcrl_dropout": [_P, _L, _P, _L, _P, _L, _L, _I, _I, _U, _U, _P, _P],
+}
+
+
 class PcrlError(RuntimeError):
     pass
 
@@ -285,6 +298,8 @@ def lib():
             pass                         # a read-only tree: the torch-first order above is what keeps this process on one runtime
         _lib = ctypes.CDLL(LIB_PATH)
         _lib.pcrl_last_error.restype = ctypes.c_char_p
+        for name, types in _SEQUENCE_ARGTYPES.items():       # declared: plain integers are passed as pointers, strides and sizes
+            getattr(_lib, name).argtypes = types
         if os.environ.get("PCRL_TRACE_LAUNCHES"):
             _lib = _TracedLib(_lib, os.environ["PCRL_TRACE_LAUNCHES"])
     return _lib

@@ -106,3 +106,14 @@ def drq_maniskill(pcd_channels=7, action_dim=22, agent_dim=68, batch_size=256, h
     cfg["actor_cfg"]["nn_cfg"]["mlp_cfg"]["zero_out_indices"] = slice(action_dim, None, None)
     cfg["actor_cfg"]["nn_cfg"]["visual_nn_cfg"]["compute_dtype"] = encoder_dtype
     return cfg
+
+
+def recurrent(cfg, **core):
+    """`cfg` (sac_dmc / sac_maniskill) with a SelectiveSSM core shared by actor and Q heads, trained by the critic's loss like the encoder; core:
+    SelectiveSSM's keywords.  Such an agent is updated from a T-step replay (DeviceReplay(sampling_cfg=dict(type="TStepTransition", horizon=H)))."""
+    from copy import deepcopy
+    cfg = deepcopy(cfg)
+    nn_cfg = cfg["actor_cfg"]["nn_cfg"]
+    nn_cfg["rnn_cfg"] = dict(type="SelectiveSSM", feat_dim=nn_cfg["mlp_cfg"]["mlp_spec"][0], **core)
+    cfg["actor_cfg"]["optim_cfg"]["param_cfg"]["(.*?)rnn(.*?)"] = None
+    return cfg

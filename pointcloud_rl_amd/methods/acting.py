@@ -30,7 +30,7 @@ class FusedActor:
         enc, mlp, head = getattr(bb, "visual_nn", None), getattr(bb, "final_mlp", None), getattr(actor, "head", None)
         if not isinstance(enc, PointNet) or enc.final_mlp is None or not isinstance(mlp, LinearMLP) or not isinstance(head, TanhGaussianHead):
             return False
-        if actor.final_mlp is not None or bb.ac_feat is not None or bb.obs_feat is not None:
+        if actor.final_mlp is not None or bb.ac_feat is not None or bb.obs_feat is not None or getattr(bb, "rnn", None) is not None or mlp.drop_p:
             return False
         if enc.mlp_spec[-1] > 256:          # the feature-head epilogue of the encoder launch is built for c3 <= 256
             return False

@@ -58,6 +58,8 @@ class DrQ(SAC):
 
     def __init__(self, num_aug=2, obs_aug=None, svea=False, inference_aug=None, *args, **kwargs):
         super().__init__(*args, **kwargs)
+        if self.is_recurrent:
+            raise NotImplementedError("DrQ's augmentations repeat single transitions; a recurrent core is trained with SAC")
         if svea:
             assert num_aug == 1, "SVEA only needs num_aug=1"          # drq.py:24-25 (FusedStep.supported declines such an agent)
         self.num_aug, self.svea = num_aug, svea

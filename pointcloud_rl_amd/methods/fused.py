@@ -130,6 +130,8 @@ class FusedStep:
     def supported(agent):
         from .sac import HipAdam
         enc = agent.encoder
+        if agent.is_recurrent or any(getattr(m, "drop_p", 0.0) for m in agent.modules()):       # a recurrent core, dropout in a head: autograd
+            return False
         if getattr(agent, "svea", False):        # DrQ(svea=True): [aug, plain] pairs against one target per pair (drq.py:62-88)
             return False
         if not isinstance(enc, PointNet) or enc.final_mlp is None or not agent._dedup or not agent.detach_actor_feature:

@@ -251,7 +251,7 @@ class SAC(BaseAgent):
         self.critic_optim = build_optimizer(self.critic, critic_optim_cfg)
         shared_target_backbone = shared_backbone if shared_target_backbone is None else shared_target_backbone
         self.target_critic = build_target_network(critic_cfg, self.critic, self.actor, shared_target_backbone)
-        self.is_recurrent = False
+        self.is_recurrent = bool(self.actor.is_recurrent)       # a recurrent core in the backbone (Visuomotor rnn_cfg)
 
         self.log_alpha = nn.Parameter(torch.ones(1, requires_grad=True))
         self.log_alpha.data *= float(np.log(np.float32(alpha)))
@@ -575,6 +575,9 @@ class SAC(BaseAgent):
         """SAC step on a device-resident batch; returns the dict of device scalars for the metrics."""
         if self._fused is not None:
             return self._fused.run(batch["obs"], batch["next_obs"], batch["actions"], batch["rewards"], batch["dones"], do_actor, polyak)
+        if self.is_recurrent:
+            from .recurrent import recurrent_step
+            return recurrent_step(self, batch, do_actor, polyak)
         stats = {}
         q_target = self._q_target(batch["next_obs"], batch["rewards"], batch["dones"])
         self._critic_step(batch["obs"], batch["actions"], q_target, stats, polyak=polyak)
@@ -641,7 +644,7 @@ class SAC(BaseAgent):
         do_actor = updates % self.actor_update_interval == 0
         polyak = self._polyak_now(updates)
         exchanging = self._be_data_parallel and exchange_active()
-        graphable = getattr(self, "_use_graphs", False) and (not (updates % self.target_update_interval == 0) or polyak) \
+        graphable = getattr(self, "_use_graphs", False) and not self.is_recurrent and (not (updates % self.target_update_interval == 0) or polyak) \
             and (not exchanging or self._fused is not None)
         if not graphable:
             stats = self._step_body(fetch(), do_actor, polyak)

@@ -17,6 +17,9 @@ class ActorCriticBase(ExtendedModule):
 
     def forward(self, obs, actions=None, *, rnn_mode="base", **kwargs):
         feature = self.backbone(obs, actions, rnn_mode=rnn_mode, **kwargs)
+        states = None
+        if self.is_recurrent and rnn_mode == "with_states":
+            feature, states = feature
         kwargs.pop("feature", None)
         if self.final_mlp is not None:
             feature = self.final_mlp(feature)
@@ -25,7 +28,7 @@ class ActorCriticBase(ExtendedModule):
         if rnn_mode == "base":
             return feature
         # non-recurrent network asked for states: None ("with_states") or [None]*3 ("full_states")
-        return feature, ([None] * 3 if rnn_mode == "full_states" else None)
+        return feature, ([None] * 3 if rnn_mode == "full_states" else states)
 
 
 def _is_box(space):

@@ -14,37 +14,30 @@ lengths [B] (integers): row b has lengths[b] steps; outputs and gradients behind
 last state is the one after step lengths[b] - 1.
 """
 import ctypes
+from ctypes import byref
 
 import torch
 
-from . import _lib
+from . import _lib, hip
 from ._lib import ConvDesc, SsmDesc, SsmGrads, check, lib
-from .hip import _span
 
 _DTYPES = {torch.float32: _lib.DT_F32, torch.bfloat16: _lib.DT_BF16, torch.float16: _lib.DT_F16}
 _getDevice, _getStream = torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream
+_empty_like = torch.empty_like
 
 
-class _NoGuard:
-    def __enter__(self):
-        return self
-
-    def __exit__(self, *exc):
-        pass
-
-
-_NO_GUARD = _NoGuard()
-
-
-def _on(t):
-    """Context in which launches go to t's device (torch's current stream there)."""
+def _on_gpu(t):
     if not t.is_cuda:
         raise RuntimeError(f"the sequence operators run on the MI355X (got a tensor on {t.device}); there is no CPU path")
-    return _NO_GUARD if t.device.index == _getDevice() else torch.cuda.device(t.device)
 
 
-def _stream():
-    return ctypes.c_void_p(_getStream(_getDevice()))
+def _launch(name, device, fn, *args):
+    """fn(*args, stream) on `device` (an index) and torch's current stream there."""
+    if hip.TIMER is None and device == _getDevice():
+        check(fn(*args, _getStream(device)))
+    else:
+        with torch.cuda.device(device), hip._span(name):
+            check(fn(*args, _getStream(device)))
 
 
 def _at(t):
@@ -126,9 +119,8 @@ def _conv_forward(x, weight, bias, state, starts, lengths, silu):
     y = torch.empty((B, T, D), dtype=x.dtype, device=x.device)
     last = torch.empty((B, weight.shape[1] - 1, D), dtype=x.dtype, device=x.device)
     if y.numel():
-        with _on(x), _span("short_conv_fwd"):
-            check(lib().pcrl_short_conv_fwd(ctypes.byref(_conv_desc(x, weight, bias, state, starts, lengths, silu, T)), ctypes.c_void_p(y.data_ptr()),
-                                            ctypes.c_void_p(last.data_ptr()), _stream()))
+        desc = _conv_desc(x, weight, bias, state, starts, lengths, silu, T)
+        _launch("short_conv_fwd", x.device.index, lib().pcrl_short_conv_fwd, byref(desc), y.data_ptr(), last.data_ptr())
     elif state is not None:
         last.copy_(state)
     else:
@@ -147,25 +139,26 @@ class _ShortConv(torch.autograd.Function):
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dy, dlast):
-        x, weight, bias, state, starts, lengths = ctx.saved_tensors
         if dy is None and dlast is None:
             return (None,) * 7
+        x, weight, bias, state, starts, lengths = ctx.saved_tensors
         B, T, D = x.shape
         dx = torch.empty((B, T, D), dtype=x.dtype, device=x.device)
-        dweight = torch.empty_like(weight, memory_format=torch.contiguous_format)
-        dbias = torch.empty_like(bias) if bias is not None else None
-        dstate = torch.empty_like(state) if state is not None else None
-        dy = torch.zeros(D, dtype=x.dtype, device=x.device).expand(B, T, D) if dy is None else dy if dy.stride(-1) == 1 else dy.contiguous()
-        dlast = dlast.contiguous() if dlast is not None else None
+        dweight = _empty_like(weight)
+        dbias = _empty_like(bias) if bias is not None else None
+        dstate = _empty_like(state) if state is not None else None
+        if dy is None:
+            dy = torch.zeros(D, dtype=x.dtype, device=x.device).expand(B, T, D)
+        elif dy.stride(2) != 1:
+            dy = dy.contiguous()
+        if dlast is not None and not dlast.is_contiguous():
+            dlast = dlast.contiguous()
         if x.numel():
-            desc, need = _conv_desc(x, weight, bias, state, starts, lengths, ctx.silu, T), ctypes.c_size_t()
-            with _on(x), _span("short_conv_bwd"):
-                check(lib().pcrl_short_conv_bwd_workspace_bytes(ctypes.byref(desc), ctypes.byref(need)))
-                work = torch.empty(need.value, dtype=torch.uint8, device=x.device)
-                check(lib().pcrl_short_conv_bwd(ctypes.byref(desc), ctypes.c_void_p(dy.data_ptr()), ctypes.c_int64(dy.stride(0)), ctypes.c_int64(dy.stride(1)),
-                                                ctypes.c_void_p(_at(dlast)), ctypes.c_void_p(dx.data_ptr()), ctypes.c_void_p(dweight.data_ptr()),
-                                                ctypes.c_void_p(_at(dbias)), ctypes.c_void_p(_at(dstate)), ctypes.c_void_p(work.data_ptr()),
-                                                ctypes.c_size_t(need.value), _stream()))
+            desc, need, fn = _conv_desc(x, weight, bias, state, starts, lengths, ctx.silu, T), ctypes.c_size_t(), lib()
+            check(fn.pcrl_short_conv_bwd_workspace_bytes(byref(desc), byref(need)))
+            work = torch.empty(need.value, dtype=torch.uint8, device=x.device)
+            _launch("short_conv_bwd", x.device.index, fn.pcrl_short_conv_bwd, byref(desc), dy.data_ptr(), dy.stride(0), dy.stride(1), _at(dlast),
+                    dx.data_ptr(), dweight.data_ptr(), _at(dbias), _at(dstate), work.data_ptr(), need.value)
         else:                                                   # no step: the state passes through
             dweight.zero_()
             if dbias is not None:
@@ -181,6 +174,7 @@ def short_conv(x, weight, bias=None, state=None, starts=None, lengths=None, acti
     x [B, T, D]; weight [D, W], bias [D] float32; state [B, W - 1, D] of x's type: the inputs in front of this call, oldest first (default:
     zeros); starts, lengths: see the module.  Returns (y [B, T, D], last_state [B, W - 1, D]); differentiable in x, weight, bias and state."""
     args = _conv_checked(x, weight, bias, state, starts, lengths, activation, 3)
+    _on_gpu(x)
     if _wants_grad(*args[:4]):
         return _ShortConv.apply(*args)
     return _conv_forward(*args)
@@ -192,11 +186,11 @@ def short_conv_step(x, state, weight, bias=None, starts=None, activation="silu",
     not overlap it); starts [B]: rows whose sequence begins here.  Not differentiable."""
     x, weight, bias, state, starts, _, silu = _conv_checked(x, weight, bias, state, starts, None, activation, 2)
     out = _state_out(state, state_out)
+    _on_gpu(x)
     y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
     if y.numel():
-        with _on(x), _span("short_conv_step"):
-            check(lib().pcrl_short_conv_fwd(ctypes.byref(_conv_desc(x, weight, bias, state, starts, None, silu, 1)), ctypes.c_void_p(y.data_ptr()),
-                                            ctypes.c_void_p(out.data_ptr()), _stream()))
+        desc = _conv_desc(x, weight, bias, state, starts, None, silu, 1)
+        _launch("short_conv_step", x.device.index, lib().pcrl_short_conv_fwd, byref(desc), y.data_ptr(), out.data_ptr())
     return y
 
 
@@ -247,31 +241,31 @@ def _ssm_checked(u, dt, A, B, C, D, z, dt_bias, state, starts, lengths, dims):
 
 def _ssm_desc(u, dt, A, B, C, D, z, dt_bias, state, starts, lengths, softplus):
     step = u.dim() == 2
-    T = 1 if step else u.shape[1]
-    st = (lambda t: 0) if step else (lambda t: t.stride(1))
-    return SsmDesc(u.shape[0], T, u.shape[-1], A.shape[1], B.shape[-2], _DTYPES[u.dtype], int(softplus), 0, u.data_ptr(), dt.data_ptr(), _at(z),
-                   u.stride(0), st(u), dt.stride(0), st(dt), z.stride(0) if z is not None else 0, st(z) if z is not None else 0,
-                   B.data_ptr(), C.data_ptr(), B.stride(0), st(B), B.stride(-2), C.stride(0), st(C), C.stride(-2),
+    if step:
+        T, su, sd, sz, sb, sc = 1, u.stride(), dt.stride(), z.stride() if z is not None else (0,), B.stride(), C.stride()
+        su, sd, sz, sb, sc = (su[0], 0), (sd[0], 0), (sz[0], 0), (sb[0], 0, sb[1]), (sc[0], 0, sc[1])
+    else:
+        T, su, sd, sz, sb, sc = u.shape[1], u.stride(), dt.stride(), z.stride() if z is not None else (0, 0), B.stride(), C.stride()
+    return SsmDesc(u.shape[0], T, u.shape[-1], A.shape[1], B.shape[-2], _DTYPES[u.dtype], softplus, 0, u.data_ptr(), dt.data_ptr(), _at(z),
+                   su[0], su[1], sd[0], sd[1], sz[0], sz[1], B.data_ptr(), C.data_ptr(), sb[0], sb[1], sb[2], sc[0], sc[1], sc[2],
                    A.data_ptr(), _at(D), _at(dt_bias), _at(state), _at(starts), T, _at(lengths))
 
 
 def _ssm_forward(args, softplus, keep):
+    """(y, last state, what a backward needs: the kept states and the size of its workspace)"""
     u, A, state = args[0], args[2], args[8]
     B, T, D = u.shape
-    N = A.shape[1]
     y = torch.empty((B, T, D), dtype=u.dtype, device=u.device)
-    last = torch.empty((B, D, N), dtype=torch.float32, device=u.device)
+    last = torch.empty((B, D, A.shape[1]), dtype=torch.float32, device=u.device)
     if not y.numel():
         last.copy_(state) if state is not None else last.zero_()
-        return y, last, None
-    desc, need, kept = _ssm_desc(*args, softplus), ctypes.c_size_t(), ctypes.c_size_t()
-    with _on(u), _span("ssm_scan_fwd"):
-        check(lib().pcrl_ssm_scan_bytes(ctypes.byref(desc), ctypes.byref(need), ctypes.byref(kept), None))
-        work = torch.empty(need.value, dtype=torch.uint8, device=u.device) if need.value else None
-        saved = torch.empty(kept.value // 4, dtype=torch.float32, device=u.device) if keep else None
-        check(lib().pcrl_ssm_scan_fwd(ctypes.byref(desc), ctypes.c_void_p(y.data_ptr()), ctypes.c_void_p(last.data_ptr()), ctypes.c_void_p(_at(saved)),
-                                      ctypes.c_void_p(_at(work)), need, _stream()))
-    return y, last, saved
+        return y, last, None, 0
+    desc, need, kept, bwd, fn = _ssm_desc(*args, softplus), ctypes.c_size_t(), ctypes.c_size_t(), ctypes.c_size_t(), lib()
+    check(fn.pcrl_ssm_scan_bytes(byref(desc), byref(need), byref(kept), byref(bwd)))
+    work = torch.empty(need.value, dtype=torch.uint8, device=u.device) if need.value else None
+    saved = torch.empty(kept.value // 4, dtype=torch.float32, device=u.device) if keep else None
+    _launch("ssm_scan_fwd", u.device.index, fn.pcrl_ssm_scan_fwd, byref(desc), y.data_ptr(), last.data_ptr(), _at(saved), _at(work), need.value)
+    return y, last, saved, bwd.value
 
 
 class _SsmScan(torch.autograd.Function):
@@ -279,31 +273,35 @@ class _SsmScan(torch.autograd.Function):
     def forward(ctx, softplus, *args):
         ctx.set_materialize_grads(False)
         ctx.softplus = softplus
-        y, last, saved = _ssm_forward(args, softplus, True)
+        y, last, saved, ctx.work_bytes = _ssm_forward(args, softplus, True)
         ctx.save_for_backward(*args, saved)
         return y, last
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dy, dlast):
-        *args, saved = ctx.saved_tensors
-        u, dt, A, B, C, D, z, dt_bias, state, starts, lengths = args
         if dy is None and dlast is None:
             return (None,) * 12
+        *args, saved = ctx.saved_tensors
+        u, dt, A, B, C, D, z, dt_bias, state = args[:9]
         shape, dev = u.shape, u.device
-        dense = lambda t: torch.empty(t.shape, dtype=t.dtype, device=dev) if t is not None else None
-        du, ddt, dA, dB, dC, dD, dz, dbias, dstate = (dense(t) for t in args[:9])
-        dy = torch.zeros(shape[2], dtype=u.dtype, device=dev).expand(shape) if dy is None else dy if dy.stride(-1) == 1 else dy.contiguous()
-        dlast = dlast.contiguous() if dlast is not None else None
+        dense = u.is_contiguous()
+        full = (lambda t: _empty_like(t)) if dense and dt.is_contiguous() and (z is None or z.is_contiguous()) else \
+            (lambda t: torch.empty(shape, dtype=u.dtype, device=dev))
+        du, ddt, dz = full(u), full(dt), full(z) if z is not None else None
+        dB, dC = torch.empty(B.shape, dtype=u.dtype, device=dev), torch.empty(C.shape, dtype=u.dtype, device=dev)
+        dA, dD, dbias, dstate = _empty_like(A), *((_empty_like(t) if t is not None else None) for t in (D, dt_bias, state))
+        if dy is None:
+            dy = torch.zeros(shape[2], dtype=u.dtype, device=dev).expand(shape)
+        elif dy.stride(2) != 1 or dy.stride(1) < 0:
+            dy = dy.contiguous()
+        if dlast is not None and not dlast.is_contiguous():
+            dlast = dlast.contiguous()
         if u.numel():
-            desc, need = _ssm_desc(*args, ctx.softplus), ctypes.c_size_t()
             grads = SsmGrads(du.data_ptr(), ddt.data_ptr(), _at(dz), dB.data_ptr(), dC.data_ptr(), dA.data_ptr(), _at(dD), _at(dbias), _at(dstate))
-            with _on(u), _span("ssm_scan_bwd"):
-                check(lib().pcrl_ssm_scan_bytes(ctypes.byref(desc), None, None, ctypes.byref(need)))
-                work = torch.empty(need.value, dtype=torch.uint8, device=dev)
-                check(lib().pcrl_ssm_scan_bwd(ctypes.byref(desc), ctypes.c_void_p(saved.data_ptr()), ctypes.c_void_p(dy.data_ptr()), ctypes.c_int64(dy.stride(0)),
-                                              ctypes.c_int64(dy.stride(1)), ctypes.c_void_p(_at(dlast)), ctypes.byref(grads), ctypes.c_void_p(work.data_ptr()),
-                                              need, _stream()))
+            work = torch.empty(ctx.work_bytes, dtype=torch.uint8, device=dev)
+            _launch("ssm_scan_bwd", dev.index, lib().pcrl_ssm_scan_bwd, byref(_ssm_desc(*args, ctx.softplus)), saved.data_ptr(), dy.data_ptr(),
+                    dy.stride(0), dy.stride(1), _at(dlast), byref(grads), work.data_ptr(), ctx.work_bytes)
         else:                                                   # no step: the state passes through
             for t in (du, ddt, dA, dB, dC, dD, dz, dbias):
                 if t is not None:
@@ -323,9 +321,10 @@ def ssm_scan(u, dt, A, B, C, D=None, z=None, dt_bias=None, softplus=True, state=
     dt_bias [D], state [B, D, N] (default: zeros) float32; starts, lengths: see the module.  Returns (y [B, T, D], last_state [B, D, N]);
     differentiable in all of them.  A call that will be differentiated keeps the state in front of every 16th step (N / 4 bytes an element)."""
     args = _ssm_checked(u, dt, A, B, C, D, z, dt_bias, state, starts, lengths, 3)
+    _on_gpu(u)
     if _wants_grad(*args[:9]):
-        return _SsmScan.apply(bool(softplus), *args)
-    return _ssm_forward(args, bool(softplus), False)[:2]
+        return _SsmScan.apply(int(bool(softplus)), *args)
+    return _ssm_forward(args, int(bool(softplus)), False)[:2]
 
 
 @torch.no_grad()
@@ -337,10 +336,10 @@ def ssm_step(u, dt, A, B, C, state, D=None, z=None, dt_bias=None, softplus=True,
     out = _state_out(state, state_out)
     if state.shape != (u.shape[0], u.shape[1], A.shape[1]) or state.dtype != torch.float32 or state.device != u.device:
         raise ValueError(f"state is {state.dtype} {tuple(state.shape)} on {state.device}, expected float32 {(u.shape[0], u.shape[1], A.shape[1])} on {u.device}")
+    _on_gpu(u)
     y = torch.empty(u.shape, dtype=u.dtype, device=u.device)
     if y.numel():
-        with _on(u), _span("ssm_step"):
-            check(lib().pcrl_ssm_step(ctypes.byref(_ssm_desc(*args, softplus)), ctypes.c_void_p(y.data_ptr()), ctypes.c_void_p(out.data_ptr()), _stream()))
+        _launch("ssm_step", u.device.index, lib().pcrl_ssm_step, byref(_ssm_desc(*args, int(bool(softplus)))), y.data_ptr(), out.data_ptr())
     return y
 
 
@@ -373,10 +372,8 @@ def _dropout(x, residual, threshold, seed, offset):
             ld = cols if x.is_contiguous() else ld
             res_ld = cols if residual.is_contiguous() else res_ld
     at = offset if torch.is_tensor(offset) else None
-    with _on(out), _span("dropout"):
-        check(lib().pcrl_dropout(ctypes.c_void_p(x.data_ptr()), ctypes.c_int64(ld), ctypes.c_void_p(_at(residual)), ctypes.c_int64(res_ld),
-                                 ctypes.c_void_p(out.data_ptr()), ctypes.c_int64(rows), ctypes.c_int64(cols), _DTYPES[out.dtype], threshold,
-                                 ctypes.c_uint64(seed), ctypes.c_uint64(0 if at is not None else offset), ctypes.c_void_p(_at(at)), _stream()))
+    _launch("dropout", out.device.index, lib().pcrl_dropout, x.data_ptr(), ld, _at(residual), res_ld, out.data_ptr(), rows, cols, _DTYPES[out.dtype],
+            threshold, seed, 0 if at is not None else offset, _at(at))
     return out
 
 
@@ -410,8 +407,7 @@ def dropout(x, p, seed, offset=0, residual=None):
         raise ValueError(f"residual is {residual.dtype} {tuple(residual.shape)} on {residual.device}, x is {x.dtype} {tuple(x.shape)} on {x.device}")
     if torch.is_tensor(offset) and (offset.dtype != torch.int64 or offset.numel() != 1 or offset.device != x.device):
         raise ValueError("offset: an integer, or an int64 tensor of one element on the device of x")
-    if not x.is_cuda:
-        _on(x)
+    _on_gpu(x)
     threshold, seed = int(round(65536.0 * p)), int(seed) & 0xFFFFFFFFFFFFFFFF
     offset = offset if torch.is_tensor(offset) else int(offset) & 0xFFFFFFFFFFFFFFFF
     if _wants_grad(x, residual):

@@ -216,8 +216,9 @@ class BaseAgent(ExtendedModule):
     def forward(self, obs, **kwargs):
         obs = to_torch(obs, device=self.device, non_blocking=True)
         kwargs = dict(kwargs)
-        if "prev_actions" in kwargs:
-            kwargs["prev_actions"] = to_torch(kwargs["prev_actions"], device=self.device, non_blocking=True)
+        for key in ("prev_actions", "rnn_states", "episode_dones"):
+            if kwargs.get(key) is not None:
+                kwargs[key] = to_torch(kwargs[key], device=self.device, non_blocking=True)
         if self.obs_processor is not None:
             obs = self.obs_processor({"obs": obs})["obs"]
         return self.actor(obs, **kwargs)
