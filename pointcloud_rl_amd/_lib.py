@@ -11,7 +11,7 @@ LIB_PATH = os.environ.get("PCRL_HIP_LIB") or os.path.join(_HERE, "libpcrl_hip.so
 
 PCRL_MAX_SEG = 4
 PCRL_MAX_CHANNELS = 16
-DT_F32, DT_U8, DT_BOOL, DT_BF16, DT_F16 = 0, 1, 2, 3, 4
+DT_F32, DT_U8, DT_BOOL = 0, 1, 2
 AUG_JITTER, AUG_AFFINE, AUG_SUBSAMPLE, AUG_COLOR = 1, 2, 4, 8
 
 
@@ -91,42 +91,6 @@ class GemmDesc(ctypes.Structure):
                 ("bias_batch_stride", ctypes.c_int64), ("mask_batch_stride", ctypes.c_int64),
                 ("relu", ctypes.c_int32), ("ones_col", ctypes.c_int32), ("accumulate", ctypes.c_int32), ("_pad", ctypes.c_int32),
                 ("C_ones", ctypes.c_void_p), ("c_ones_batch_stride", ctypes.c_int64)]
-
-
-class ConvDesc(ctypes.Structure):
-    _fields_ = [("B", ctypes.c_int32), ("T", ctypes.c_int32), ("D", ctypes.c_int32), ("W", ctypes.c_int32), ("dtype", ctypes.c_int32),
-                ("silu", ctypes.c_int32), ("x", ctypes.c_void_p), ("x_sb", ctypes.c_int64), ("x_st", ctypes.c_int64), ("weight", ctypes.c_void_p),
-                ("bias", ctypes.c_void_p), ("state", ctypes.c_void_p), ("starts", ctypes.c_void_p), ("starts_sb", ctypes.c_int64),
-                ("lengths", ctypes.c_void_p)]
-
-
-class SsmDesc(ctypes.Structure):
-    _fields_ = [("B", ctypes.c_int32), ("T", ctypes.c_int32), ("D", ctypes.c_int32), ("N", ctypes.c_int32), ("G", ctypes.c_int32),
-                ("dtype", ctypes.c_int32), ("softplus", ctypes.c_int32), ("_pad", ctypes.c_int32),
-                ("u", ctypes.c_void_p), ("dt", ctypes.c_void_p), ("z", ctypes.c_void_p),
-                ("u_sb", ctypes.c_int64), ("u_st", ctypes.c_int64), ("dt_sb", ctypes.c_int64), ("dt_st", ctypes.c_int64),
-                ("z_sb", ctypes.c_int64), ("z_st", ctypes.c_int64), ("Bm", ctypes.c_void_p), ("Cm", ctypes.c_void_p),
-                ("b_sb", ctypes.c_int64), ("b_st", ctypes.c_int64), ("b_sg", ctypes.c_int64),
-                ("c_sb", ctypes.c_int64), ("c_st", ctypes.c_int64), ("c_sg", ctypes.c_int64),
-                ("A", ctypes.c_void_p), ("D_skip", ctypes.c_void_p), ("dt_bias", ctypes.c_void_p), ("state", ctypes.c_void_p),
-                ("starts", ctypes.c_void_p), ("starts_sb", ctypes.c_int64), ("lengths", ctypes.c_void_p)]
-
-
-class SsmGrads(ctypes.Structure):
-    _fields_ = [(k, ctypes.c_void_p) for k in ("du", "ddt", "dz", "dB", "dC", "dA", "dD", "ddt_bias", "dstate")]
-
-
-_P, _I, _L, _Z, _U = ctypes.c_void_p, ctypes.c_int32, ctypes.c_int64, ctypes.c_size_t, ctypes.c_uint64
-_SEQUENCE_ARGTYPES = {
-    "pcrl_short_conv_fwd": [_P, _P, _P, _P],
-    "pcrl_short_conv_bwd_workspace_bytes": [_P, _P],
-    "pcrl_short_conv_bwd": [_P, _P, _L, _L, _P, _P, _P, _P, _P, _P, _Z, _P],
-    "pcrl_ssm_scan_bytes": [_P, _P, _P, _P],
-    "pcrl_ssm_scan_fwd": [_P, _P, _P, _P, _P, _Z, _P],
-    "pcrl_ssm_scan_bwd": [_P, _P, _P, _L, _L, _P, _P, _P, _Z, _P],
-    "pcrl_ssm_step": [_P, _P, _P, _P],
-    "pcrl_dropout": [_P, _L, _P, _L, _P, _L, _L, _I, _I, _U, _U, _P, _P],
-}
 
 
 class PcrlError(RuntimeError):
@@ -298,11 +262,34 @@ def lib():
             pass                         # a read-only tree: the torch-first order above is what keeps this process on one runtime
         _lib = ctypes.CDLL(LIB_PATH)
         _lib.pcrl_last_error.restype = ctypes.c_char_p
-        for name, types in _SEQUENCE_ARGTYPES.items():       # declared: plain integers are passed as pointers, strides and sizes
-            getattr(_lib, name).argtypes = types
         if os.environ.get("PCRL_TRACE_LAUNCHES"):
             _lib = _TracedLib(_lib, os.environ["PCRL_TRACE_LAUNCHES"])
     return _lib
+
+
+_sequence = None
+SEQUENCE_PATH = os.path.join(_HERE, "_sequence.so")
+_SEQUENCE_ENTRIES = ("pcrl_last_error", "pcrl_short_conv_fwd", "pcrl_short_conv_bwd_workspace_bytes", "pcrl_short_conv_bwd", "pcrl_ssm_scan_bytes",
+                     "pcrl_ssm_scan_fwd", "pcrl_ssm_scan_bwd", "pcrl_ssm_step", "pcrl_dropout")
+
+
+def sequence_ext():
+    """The torch binding of the sequence operators (csrc/torch_binding.cpp), loaded once and handed the addresses of libpcrl_hip.so's entry
+    points.  Raises if it has not been built.  Its launches do not pass through the ctypes binding, so PCRL_TRACE_LAUNCHES does not see them."""
+    global _sequence
+    if _sequence is None:
+        import importlib.util
+        dll = lib()                      # torch first, then the kernels
+        if not os.path.exists(SEQUENCE_PATH):
+            raise PcrlError(f"{SEQUENCE_PATH} is missing: build the HIP extension first "
+                            "(python -c 'import __graft_entry__ as g; g.build()' or make -C pointcloud_rl_amd/csrc)")
+        spec = importlib.util.spec_from_file_location("_sequence", SEQUENCE_PATH)
+        ext = importlib.util.module_from_spec(spec)
+        spec.loader.exec_module(ext)
+        dll = dll.__dict__.get("_cdll", dll)
+        ext.bind({name: ctypes.cast(getattr(dll, name), ctypes.c_void_p).value for name in _SEQUENCE_ENTRIES})
+        _sequence = ext
+    return _sequence
 
 
 def check(rc):

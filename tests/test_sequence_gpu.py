@@ -30,6 +30,30 @@ def close(name, got, want, mag, k):
     assert not bad.any(), f"{name}: {int(bad.sum())} of {bad.numel()} off, worst {float((err / tol.clamp(min=1e-300)).nan_to_num(1e9).max()):.3g} times the bound"
 
 
+# ctypes mirrors of the sequence descriptors of include/pcrl.h, for calls of the C entry points themselves
+class ConvDesc(ctypes.Structure):
+    _fields_ = [("B", ctypes.c_int32), ("T", ctypes.c_int32), ("D", ctypes.c_int32), ("W", ctypes.c_int32), ("dtype", ctypes.c_int32),
+                ("silu", ctypes.c_int32), ("x", ctypes.c_void_p), ("x_sb", ctypes.c_int64), ("x_st", ctypes.c_int64), ("weight", ctypes.c_void_p),
+                ("bias", ctypes.c_void_p), ("state", ctypes.c_void_p), ("starts", ctypes.c_void_p), ("starts_sb", ctypes.c_int64),
+                ("lengths", ctypes.c_void_p)]
+
+
+class SsmDesc(ctypes.Structure):
+    _fields_ = [("B", ctypes.c_int32), ("T", ctypes.c_int32), ("D", ctypes.c_int32), ("N", ctypes.c_int32), ("G", ctypes.c_int32),
+                ("dtype", ctypes.c_int32), ("softplus", ctypes.c_int32), ("_pad", ctypes.c_int32),
+                ("u", ctypes.c_void_p), ("dt", ctypes.c_void_p), ("z", ctypes.c_void_p),
+                ("u_sb", ctypes.c_int64), ("u_st", ctypes.c_int64), ("dt_sb", ctypes.c_int64), ("dt_st", ctypes.c_int64),
+                ("z_sb", ctypes.c_int64), ("z_st", ctypes.c_int64), ("Bm", ctypes.c_void_p), ("Cm", ctypes.c_void_p),
+                ("b_sb", ctypes.c_int64), ("b_st", ctypes.c_int64), ("b_sg", ctypes.c_int64),
+                ("c_sb", ctypes.c_int64), ("c_st", ctypes.c_int64), ("c_sg", ctypes.c_int64),
+                ("A", ctypes.c_void_p), ("D_skip", ctypes.c_void_p), ("dt_bias", ctypes.c_void_p), ("state", ctypes.c_void_p),
+                ("starts", ctypes.c_void_p), ("starts_sb", ctypes.c_int64), ("lengths", ctypes.c_void_p)]
+
+
+class SsmGrads(ctypes.Structure):
+    _fields_ = [(k, ctypes.c_void_p) for k in ("du", "ddt", "dz", "dB", "dC", "dA", "dD", "ddt_bias", "dstate")]
+
+
 # ---- scan ------------------------------------------------------------------------------------------------------------------------------------
 def scan_inputs(dev, dtype, Bt, T, Dm, N, G=1, z=True, skip=True, bias=True, state=True, starts=0.0, lengths=None, seed=0):
     g = torch.Generator().manual_seed(seed)
@@ -523,13 +547,13 @@ def test_the_c_entry_points_refuse_bad_descriptors():
     n = ctypes.c_size_t()
 
     def ssm(**kw):
-        d = _lib.SsmDesc(B=1, T=2, D=8, N=4, G=1, u=4096, dt=4096, Bm=4096, Cm=4096, A=4096)
+        d = SsmDesc(B=1, T=2, D=8, N=4, G=1, u=4096, dt=4096, Bm=4096, Cm=4096, A=4096)
         for k, v in kw.items():
             setattr(d, k, v)
         return ctypes.byref(d)
 
     def conv(**kw):
-        d = _lib.ConvDesc(B=1, T=2, D=8, W=4, x=4096, weight=4096)
+        d = ConvDesc(B=1, T=2, D=8, W=4, x=4096, weight=4096)
         for k, v in kw.items():
             setattr(d, k, v)
         return ctypes.byref(d)
@@ -540,7 +564,7 @@ def test_the_c_entry_points_refuse_bad_descriptors():
     assert lib.pcrl_ssm_scan_fwd(None, one, None, None, None, ctypes.c_size_t(0), None) == -1
     assert lib.pcrl_ssm_scan_fwd(ssm(), None, None, None, None, ctypes.c_size_t(0), None) == -1
     assert lib.pcrl_ssm_scan_bwd(ssm(), one, one, ctypes.c_int64(16), ctypes.c_int64(8), None, None, one, ctypes.c_size_t(1 << 30), None) == -1
-    grads = _lib.SsmGrads(*[4096] * 9)
+    grads = SsmGrads(*[4096] * 9)
     assert lib.pcrl_ssm_scan_bwd(ssm(), one, one, ctypes.c_int64(16), ctypes.c_int64(8), None, ctypes.byref(grads), one, ctypes.c_size_t(16), None) == -2
     assert b"workspace" in lib.pcrl_last_error()
     assert lib.pcrl_ssm_step(ssm(), one, one, None) == -1 and lib.pcrl_ssm_step(ssm(T=1), one, one, None) == -1        # T = 2; no state
@@ -558,9 +582,8 @@ def test_struct_layouts_match_the_header(tmp_path):
     """sizeof / offsetof of the sequence descriptors as gcc lays them out == the ctypes mirror."""
     import os
     import subprocess
-    from pointcloud_rl_amd import _lib
     root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
-    pairs = [("pcrl_conv_desc", _lib.ConvDesc), ("pcrl_ssm_desc", _lib.SsmDesc), ("pcrl_ssm_grads", _lib.SsmGrads)]
+    pairs = [("pcrl_conv_desc", ConvDesc), ("pcrl_ssm_desc", SsmDesc), ("pcrl_ssm_grads", SsmGrads)]
     lines = []
     for cname, cls in pairs:
         lines.append(f'printf("{cname} %zu\\n", sizeof({cname}));')
