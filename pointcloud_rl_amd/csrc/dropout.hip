@@ -73,7 +73,7 @@ extern "C" int pcrl_dropout(const void* x, int64_t x_ld, const void* residual, i
     p.flat = (x_ld == cols || rows == 1) && (!residual || residual_ld == cols || rows == 1) &&
              ((uintptr_t)x | (uintptr_t)out | (uintptr_t)residual) % align == 0;
     const long long groups = (p.n + 7) / 8, blocks = (groups + 255) / 256;
-    if (blocks > 0x7FFFFFFFLL) return fail(PCRL_E_ARG, "pcrl_dropout: too many workgroups");
+    if (blocks > kMaxGroups) return fail(PCRL_E_ARG, "pcrl_dropout: too many workgroups");
     const dim3 grid((unsigned)blocks);
     hipStream_t s = (hipStream_t)stream;
     if (dtype == PCRL_DT_F32) dropout_kernel<float><<<grid, 256, 0, s>>>(p);

@@ -131,6 +131,7 @@ __device__ __forceinline__ float dot_row_bcast(const float (&c)[RN], const float
 }
 #undef PCRL_FMAC_ROW
 
+constexpr long long kMaxGroups = (1LL << 24) - 1;      // workgroups of 256: a grid holds fewer than 2^32 threads
 __host__ inline int elem_bytes(int dtype) { return dtype == PCRL_DT_F32 ? 4 : 2; }
 __host__ inline bool seq_dtype(int dtype) { return dtype == PCRL_DT_F32 || dtype == PCRL_DT_BF16 || dtype == PCRL_DT_F16; }
 

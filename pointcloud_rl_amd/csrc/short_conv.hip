@@ -351,6 +351,7 @@ __global__ __launch_bounds__(1024) void conv_finish_kernel(const float* part, in
 static int conv_check(const pcrl_conv_desc* d, const char* who) {
     if (!d) return fail(PCRL_E_ARG, "%s: null descriptor", who);
     if (d->B < 1 || d->T < 1 || d->D < 1) return fail(PCRL_E_ARG, "%s: B, T, D must be positive (%d, %d, %d)", who, d->B, d->T, d->D);
+    if (d->T > 0x7FFFFFE0) return fail(PCRL_E_ARG, "%s: T = %d", who, d->T);        // (a run's end is a 32-bit step)
     if (d->W < 1 || d->W > 4) return fail(PCRL_E_ARG, "%s: W = %d taps (1 to 4)", who, d->W);
     if (!seq_dtype(d->dtype)) return fail(PCRL_E_ARG, "%s: dtype %d", who, d->dtype);
     if (!d->x || !d->weight) return fail(PCRL_E_ARG, "%s: null input", who);
@@ -375,14 +376,14 @@ static int conv_fwd(ConvParams& p, hipStream_t s) {
     const long long nvec = (p.D + V - 1) / V;
     if (p.T == 1) {
         const long long blocks = (nvec * p.B + 255) / 256;
-        if (blocks > 0x7FFFFFFFLL) return fail(PCRL_E_ARG, "pcrl_short_conv_fwd: too many workgroups");
+        if (blocks > kMaxGroups) return fail(PCRL_E_ARG, "pcrl_short_conv_fwd: too many workgroups");
         conv_step_kernel<T, V, W><<<dim3((unsigned)blocks), 256, 0, s>>>(p);
         PCRL_CHECK_LAUNCH("conv_step_kernel");
         return PCRL_OK;
     }
     p.nrun = (p.T + kRun - 1) / kRun;
     const long long blocks = (nvec * p.B * (p.nrun + 1) + 255) / 256;
-    if (blocks > 0x7FFFFFFFLL) return fail(PCRL_E_ARG, "pcrl_short_conv_fwd: too many workgroups");
+    if (blocks > kMaxGroups) return fail(PCRL_E_ARG, "pcrl_short_conv_fwd: too many workgroups");
     conv_fwd_kernel<T, V, W><<<dim3((unsigned)blocks), 256, 0, s>>>(p);
     PCRL_CHECK_LAUNCH("conv_fwd_kernel");
     return PCRL_OK;

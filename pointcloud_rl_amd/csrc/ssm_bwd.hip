@@ -277,8 +277,8 @@ __global__ __launch_bounds__(256, 2) void ssm_bwd_kernel(const SsmParams) {
                                     gc[k][j] = fresh ? 0.0f : next;
                                 }
                             }
-                            dt_sum += dt4[i];
                         });
+                        dt_sum += (dt4[0] + dt4[1]) + (dt4[2] + dt4[3]);
                     });
                 } else {
                     static_for<NG>([&](auto kc) {
@@ -556,7 +556,7 @@ extern "C" int pcrl_ssm_scan_bwd(const pcrl_ssm_desc* d, const float* saved, con
     const BwdLayout at = bwd_layout(d, plan);
     if (!workspace || workspace_bytes < at.total) return fail(PCRL_E_WORKSPACE, "pcrl_ssm_scan_bwd: workspace %zu < %zu", workspace_bytes, at.total);
     const long long elems = 2LL * d->B * d->T * d->G * d->N;
-    if ((long long)d->G * plan.nblk * plan.nchunk * d->B > 0x7FFFFFFFLL || elems / 1024 > 0x3FFFFFFFLL) return fail(PCRL_E_ARG, "pcrl_ssm_scan_bwd: too many workgroups");
+    if ((long long)d->G * plan.nblk * plan.nchunk * d->B > kMaxGroups || elems / 1024 + (long long)d->D * (d->N + 2) / 64 > kMaxGroups / 4 - 2) return fail(PCRL_E_ARG, "pcrl_ssm_scan_bwd: too many workgroups");
     float* w = (float*)workspace;
     SsmParams p;
     ssm_fill(p, d);

@@ -1,6 +1,5 @@
 // Selective state space scan, forward and single step (ssm_common.h: the split; include/pcrl.h: the formulas).
 #include "ssm_common.h"
-#include <cstdlib>
 
 namespace pcrl {
 
@@ -159,9 +158,9 @@ __global__ __launch_bounds__(256) void ssm_fwd_kernel(const SsmParams) {
                         }
                         if (!SUMMARY) acc = k == 0 ? dot_row_bcast<t, RN>(Cv[k], h[k]) : acc + dot_row_bcast<t, RN>(Cv[k], h[k]);
                     }
-                    if (SUMMARY) dt_sum += dt4[i];
-                    else s_y[q * kPartLd + t * 16 + ch] = acc;
+                    if (!SUMMARY) s_y[q * kPartLd + t * 16 + ch] = acc;
                 });
+                if (SUMMARY) dt_sum += (dt4[0] + dt4[1]) + (dt4[2] + dt4[3]);
             });
         };
         if (starts) { walk(std::true_type{}); cut = true; }
@@ -272,6 +271,7 @@ __global__ __launch_bounds__(256) void ssm_step_kernel(const SsmStepParams q) {
 // ---- host --------------------------------------------------------------------------------------------------------------------------------
 int ssm_check(const pcrl_ssm_desc* d, const char* who) {
     if (!d) return fail(PCRL_E_ARG, "%s: null descriptor", who);
+    if (d->B > (1 << 30) || d->T > 0x7FFFFFE0) return fail(PCRL_E_ARG, "%s: B = %d, T = %d", who, d->B, d->T);      // (a tile's end is a 32-bit step)
     if (d->B < 1 || d->T < 1 || d->D < 1 || d->N < 1 || d->G < 1) return fail(PCRL_E_ARG, "%s: B, T, D, N, G must be positive (%d, %d, %d, %d, %d)", who, d->B, d->T, d->D, d->N, d->G);
     if (d->N > kSsmMaxN) return fail(PCRL_E_ARG, "%s: N = %d states per channel (at most %d)", who, d->N, kSsmMaxN);
     if (d->D % d->G) return fail(PCRL_E_ARG, "%s: %d channels are not shared evenly by %d groups", who, d->D, d->G);
@@ -289,12 +289,12 @@ bool ssm_vec(const pcrl_ssm_desc* d, const void* const* extra, const long long* 
     const void* ptr[3] = {d->u, d->dt, d->z};
     const long long st[3][2] = {{d->u_sb, d->u_st}, {d->dt_sb, d->dt_st}, {d->z_sb, d->z_st}};
     for (int i = 0; i < 3; ++i)
-        if (ptr[i] && ((uintptr_t)ptr[i] % bytes || st[i][0] % 4 || st[i][1] % 4)) return false;
+        if (ptr[i] && ((uintptr_t)ptr[i] % bytes || (d->B > 1 && st[i][0] % 4) || (d->T > 1 && st[i][1] % 4))) return false;
     for (int i = 0; i < n_extra; ++i)
-        if (extra[i] && ((uintptr_t)extra[i] % bytes || strides[2 * i] % 4 || strides[2 * i + 1] % 4)) return false;
+        if (extra[i] && ((uintptr_t)extra[i] % bytes || (d->B > 1 && strides[2 * i] % 4) || (d->T > 1 && strides[2 * i + 1] % 4))) return false;
     const int rn = ssm_rn(d->N);
     return d->N % rn == 0 && ((uintptr_t)d->Bm | (uintptr_t)d->Cm) % ((uintptr_t)rn * elem_bytes(d->dtype)) == 0 &&
-           (d->b_sb | d->b_st | d->b_sg | d->c_sb | d->c_st | d->c_sg) % rn == 0;
+           ((d->B > 1 ? d->b_sb | d->c_sb : 0) | (d->T > 1 ? d->b_st | d->c_st : 0) | (d->G > 1 ? d->b_sg | d->c_sg : 0)) % rn == 0;
 }
 bool ssm_vec_n(const pcrl_ssm_desc* d, const void* const* extra, int n_extra) {
     const int rn = ssm_rn(d->N);
@@ -315,15 +315,17 @@ void ssm_fill(SsmParams& p, const pcrl_ssm_desc* d) {
     p.starts = d->starts, p.starts_sb = d->starts_sb, p.lengths = d->lengths;
 }
 
+// How many chunks.  One chunk does the walk's work once; more chunks fill the chip when there are few channel blocks, and pay a summary pass
+// (0.4 to 0.7 of the forward's walk, 0.2 to 0.3 of the backward's).  Measured on 16.8 M elements, bf16, N = 16, us (forward / backward, all launches) at 1, 2, 4, 8
+// chunks: 128 blocks 321 / 818, 262 / 492, 174 / 343, 152 / 335; 256 blocks 162 / 376, 154 / 329, 140 / 327, -; 384 blocks (25 M elements) 189 / 496,
+// 208 / 498, 208 / 482, -; 512 blocks 104 / 268, 126 / 307, 139 / 333, -.  So: none from 1.5 blocks per CU on, else up to 4 workgroups per CU forward
+// and 2 backward (its registers and LDS admit no more), down to single tiles (a 333-step batch of 28 blocks: 21 chunks 19 / 33, 7 chunks 21 / 38).
 SsmPlan ssm_plan(const pcrl_ssm_desc* d, bool backward) {
     SsmPlan plan{};
     const int ntile = cdiv(d->T, kTile);
     plan.nblk = cdiv(d->D / d->G, 64);
-    const long long blocks = (long long)d->B * d->G * plan.nblk;
-    const long long cus = num_cus();
+    const long long blocks = (long long)d->B * d->G * plan.nblk, cus = num_cus();
     long long chunks = 2 * blocks >= 3 * cus ? 1 : ((backward ? 2 : 4) * cus + blocks - 1) / blocks;
-    const char* e = getenv(backward ? "PCRL_X_BCHUNKS" : "PCRL_X_CHUNKS");
-    if (e) chunks = atoi(e);
     if (chunks > ntile) chunks = ntile;
     plan.chunk_tiles = cdiv(ntile, chunks);
     plan.nchunk = cdiv(ntile, plan.chunk_tiles);
@@ -385,7 +387,7 @@ extern "C" int pcrl_ssm_scan_fwd(const pcrl_ssm_desc* d, void* y, float* last_st
     const SsmPlan plan = ssm_plan(d, false);
     const size_t need = fwd_workspace(d, plan);
     if (need && (!workspace || workspace_bytes < need)) return fail(PCRL_E_WORKSPACE, "pcrl_ssm_scan_fwd: workspace %zu < %zu", workspace_bytes, need);
-    if ((long long)d->G * plan.nblk * plan.nchunk * d->B > 0x7FFFFFFFLL) return fail(PCRL_E_ARG, "pcrl_ssm_scan_fwd: too many workgroups");
+    if ((long long)d->G * plan.nblk * plan.nchunk * d->B > kMaxGroups) return fail(PCRL_E_ARG, "pcrl_ssm_scan_fwd: too many workgroups");
     SsmParams p;
     ssm_fill(p, d);
     p.nblk = plan.nblk, p.nchunk = plan.nchunk, p.chunk_tiles = plan.chunk_tiles;

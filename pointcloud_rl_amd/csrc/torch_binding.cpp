@@ -94,11 +94,11 @@ Tensor starts_of(const Opt& starts, at::IntArrayRef rows, const Tensor& like) {
                       "starts is ", starts->scalar_type(), " ", starts->sizes(), " on ", starts->device(), ", expected bool ", rows, " on ", like.device());
     return starts->contiguous();
 }
-Tensor lengths_of(const Opt& lengths, int64_t rows, const Tensor& like) {
+Tensor lengths_of(const Opt& lengths, int64_t rows, int64_t steps, const Tensor& like) {
     if (!lengths.has_value()) return Tensor();
     TORCH_CHECK_VALUE(lengths->dim() == 1 && lengths->size(0) == rows && (lengths->scalar_type() == at::kInt || lengths->scalar_type() == at::kLong) && lengths->device() == like.device(),
                       "lengths is ", lengths->scalar_type(), " ", lengths->sizes(), " on ", lengths->device(), ", expected int32 [", rows, "] on ", like.device());
-    return lengths->to(at::kInt).contiguous();
+    return lengths->scalar_type() == at::kInt ? lengths->contiguous() : lengths->clamp(0, steps).to(at::kInt);
 }
 bool wants_grad(std::initializer_list<Tensor> ts) {
     if (!at::GradMode::is_enabled()) return false;
@@ -184,7 +184,7 @@ ConvArgs conv_args(const Tensor& x, const Tensor& weight, const Opt& bias, const
     if (bias.has_value()) a.bias = parameter("bias", *bias, {D}, x);
     if (state.has_value()) a.state = activation("state", *state, {x.size(0), weight.size(1) - 1, D}, x);
     a.starts = starts_of(starts, x.sizes().slice(0, dims - 1), x);
-    a.lengths = lengths_of(lengths, x.size(0), x);
+    a.lengths = lengths_of(lengths, x.size(0), dims == 3 ? x.size(1) : 1, x);
     a.silu = act.has_value();
     return a;
 }
@@ -198,6 +198,9 @@ Tensor state_out_of(const Tensor& state, const Opt& out) {
     TORCH_CHECK_VALUE(a == b || a + state.nbytes() <= b || b + out->nbytes() <= a, "state_out overlaps the state");
     return *out;
 }
+
+// A graph that saved the old state must not be differentiated with the new one in its place.
+void written(const Tensor& t) { if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version(); }
 
 std::tuple<Tensor, Tensor> short_conv(const Tensor& x, const Tensor& weight, const Opt& bias, const Opt& state, const Opt& starts, const Opt& lengths,
                                       const std::optional<std::string>& act) {
@@ -220,7 +223,7 @@ Tensor short_conv_step(const Tensor& x, const Opt& state, const Tensor& weight, 
         const pcrl_conv_desc d = conv_desc(a.x, a.weight, a.bias, a.state, a.starts, Tensor(), a.silu);
         check(api.conv_fwd(&d, to_(y), to_(out), on.stream));
     }
-    out.unsafeGetTensorImpl()->bump_version();
+    written(out);
     return y;
 }
 
@@ -325,7 +328,7 @@ ScanArgs scan_args(const Tensor& u, const Tensor& dt, const Tensor& A, const Ten
     a.B = adjacent(activation("B", B.dim() == dims ? B.unsqueeze(-2) : B, shape, u), dims);
     a.C = adjacent(activation("C", C.dim() == dims ? C.unsqueeze(-2) : C, shape, u), dims);
     a.starts = starts_of(starts, u.sizes().slice(0, dims - 1), u);
-    a.lengths = lengths_of(lengths, u.size(0), u);
+    a.lengths = lengths_of(lengths, u.size(0), dims == 3 ? u.size(1) : 1, u);
     a.softplus = softplus;
     return a;
 }
@@ -352,7 +355,7 @@ Tensor ssm_step(const Tensor& u, const Tensor& dt, const Tensor& A, const Tensor
         const pcrl_ssm_desc d = scan_desc(a);
         check(api.step(&d, to_(y), (float*)to_(out), on.stream));
     }
-    out.unsafeGetTensorImpl()->bump_version();
+    written(out);
     return y;
 }
 
