@@ -1,6 +1,8 @@
 // Dropout from a counter-based generator (include/pcrl.h: which word decides which element).  The mask is a function of (seed, offset, element
 // index), so nothing is stored for the backward: it is the same launch on the gradient.
 // One Philox call decides eight elements (16 bits each: probabilities in steps of 2^-16), which is one 16-byte access of a 16-bit type.
+// All of it is 173 instructions for eight elements (11 us of every SIMD at 8192 x 2048), so memory bounds it: bf16, 13.4 us without a residual
+// (67 MB, 5.0 TB/s) and 17.7 us with one (101 MB, 5.7 TB/s, part of it from the last-level cache).
 #include "seq_common.h"
 
 namespace pcrl {

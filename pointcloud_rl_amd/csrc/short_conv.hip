@@ -1,12 +1,13 @@
 // Short causal convolution over time, one filter of W taps per channel, optional SiLU (include/pcrl.h: the formulas).
 // Bound by memory: a thread owns V adjacent channels (16 bytes) and a run of steps, keeps the last W - 1 inputs in registers and so reads every
-// input once (plus W - 1 rows of halo per run).
+// input once (plus W - 1 rows of halo per run).  4 x 2048 x 2048, W = 4, bf16: forward 16.5 us (67 MB, 4.1 TB/s; 11 us of every SIMD are vector
+// instructions), backward 27.3 us (101 MB, 3.7 TB/s; 15 us of them, at three waves per SIMD) and 4 us of sums.
 #include "seq_common.h"
 
 namespace pcrl {
 
 constexpr int kConvV = 4;                              // adjacent channels of a thread
-constexpr int kRun = 8;                                // steps a forward thread takes
+constexpr int kRun = 8;                                // steps a forward thread takes (16: 18.9 us for 17.4, half the waves)
 
 struct ConvParams {
     int B, T, D, silu, vec, vec_w, nrun, run;          // vec, vec_w: whole vectors of the activations, of the weights; runs of `run` steps (backward)
@@ -82,10 +83,14 @@ __device__ __forceinline__ void conv_weights(const ConvParams& p, int d0, int nv
 
 template <typename T, int V, int W>
 __global__ __launch_bounds__(256) void conv_fwd_kernel(const ConvParams p) {
-    const int nvec = (p.D + V - 1) / V;
-    const long long idx = (long long)blockIdx.x * 256 + threadIdx.x, line = idx / nvec;
+    // Workgroups go to the eight XCDs in turn: dealt out so that each XCD has adjacent runs, whose halo rows are then in its own L2
+    // (17.2 -> 16.5 us).
+    const unsigned xcd = blockIdx.x & 7u, some = gridDim.x >> 3, more = gridDim.x & 7u;
+    const unsigned blk = xcd * some + (xcd < more ? xcd : more) + (blockIdx.x >> 3);
+    const unsigned nvec = (unsigned)(p.D + V - 1) / V, runs = (unsigned)p.nrun + 1;      // (a grid holds fewer than 2^32 threads: 32-bit divisions)
+    const unsigned idx = blk * 256u + threadIdx.x, line = idx / nvec;
     const int d0 = (int)(idx - line * nvec) * V, nv = p.D - d0 < V ? p.D - d0 : V;
-    const int b = (int)(line / (p.nrun + 1)), q = (int)(line - (long long)b * (p.nrun + 1));
+    const int b = (int)(line / runs), q = (int)(line - (unsigned)b * runs);
     if (b >= p.B) return;
     const int len = conv_length(p, b);
     float win[W][V];
@@ -158,9 +163,8 @@ __global__ __launch_bounds__(256) void conv_fwd_kernel(const ConvParams p) {
 // One step: a thread reads the W - 1 state rows of its channels before it writes them, so the state may be updated in place.
 template <typename T, int V, int W>
 __global__ __launch_bounds__(256) void conv_step_kernel(const ConvParams p) {
-    const int nvec = (p.D + V - 1) / V;
-    const long long idx = (long long)blockIdx.x * 256 + threadIdx.x, line = idx / nvec;
-    if (line >= p.B) return;
+    const unsigned nvec = (unsigned)(p.D + V - 1) / V, idx = blockIdx.x * 256u + threadIdx.x, line = idx / nvec;
+    if (line >= (unsigned)p.B) return;
     const int b = (int)line, d0 = (int)(idx - line * nvec) * V, nv = p.D - d0 < V ? p.D - d0 : V;
     const bool on = conv_length(p, b) > 0;
     const RawVec<T, V> raw = raw_load<T, V>((const T*)p.x + b * p.x_sb + d0, on ? nv : 0, p.vec);
@@ -179,7 +183,7 @@ __global__ __launch_bounds__(256) void conv_step_kernel(const ConvParams p) {
         if (p.silu) acc *= sigmoidf_(acc);
         out[i] = on ? acc : 0.0f;
     }
-    if (p.y) raw_store<T, V>((T*)p.y + (long long)b * p.D + d0, out, nv, p.vec);
+    raw_store<T, V>((T*)p.y + (long long)b * p.D + d0, out, nv, p.vec);
     if (p.last) {
 #pragma unroll
         for (int k = 0; k < W - 1; ++k) {
@@ -191,12 +195,15 @@ __global__ __launch_bounds__(256) void conv_step_kernel(const ConvParams p) {
 
 // Backward.  A thread walks its run (and W - 1 steps behind it, whose outputs its inputs also feed): dpre of step s from the window of inputs,
 // then dx of the last W inputs gets its tap's share.  An input is complete when its W-th step has passed or a new sequence has begun.
+// Steps without tests (whole vectors, no starts) have a body of their own: 40.8 -> 29.3 us; runs of 32 instead of 16: 27.3 (of 8: 35).  A fourth
+// wave per SIMD (128 registers) spills: 38; the next group's loads ahead of this one's arithmetic: 25.9, but 12.2 -> 13.1 at 256 x 16 x 256.
 template <typename T, int V, int W>
 __global__ __launch_bounds__(256) void conv_bwd_kernel(const ConvParams p) {
     extern __shared__ float s_part[];                  // [4][W + 1][64 V]
     // a workgroup: 64 channel vectors x 4 walkers; walker (blockIdx.y, k) takes every parts-th (b, run)
     const int lane = threadIdx.x & 63, k4 = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int d0 = (blockIdx.x * 64 + lane) * V, nv = p.D - d0 < V ? p.D - d0 : V;       // nv <= 0: no channel
+    const unsigned lanes[V] = {nv > 0 ? (unsigned)d0 : 0u};             // (whole vectors only: the first element's place)
     float w[W][V], bias[V], dw[W][V], db[V];
     conv_weights<V, W>(p, d0, nv, w, bias);
 #pragma unroll
@@ -210,10 +217,10 @@ __global__ __launch_bounds__(256) void conv_bwd_kernel(const ConvParams p) {
         const int b = (int)(line / p.nrun), q = (int)(line - (long long)b * p.nrun);
         const int len = conv_length(p, b);
         const int t_first = q * p.run, t_last = t_first + p.run < p.T ? t_first + p.run : p.T;
-        const T* px = (const T*)p.x + b * p.x_sb + d0;
-        const T* pg = (const T*)p.dy + b * p.dy_sb + d0;
+        const T* px = (const T*)p.x + b * p.x_sb;
+        const T* pg = (const T*)p.dy + b * p.dy_sb;
         const uint8_t* ps = p.starts ? p.starts + b * p.starts_sb : nullptr;
-        T* dx = (T*)p.dx + (long long)b * p.T * p.D + d0;
+        T* dx = (T*)p.dx + (long long)b * p.T * p.D;
         float win[W][V], acc[W][V];                    // inputs s - (W - 1) ... s and their dx so far
         bool alive[W];                                 // ... still in the sequence of step s
 #pragma unroll
@@ -223,45 +230,46 @@ __global__ __launch_bounds__(256) void conv_bwd_kernel(const ConvParams p) {
             for (int i = 0; i < V; ++i) win[j][i] = acc[j][i] = 0.0f;
         }
         if (W > 1) conv_window<T, V, W>(p, b, d0, nv, t_first, win);
-        auto finish = [&](int t, const float (&g)[V]) {              // dx of input t is complete
-            if (t >= t_first && t < t_last) raw_store<T, V>(dx + (long long)t * p.D, g, nv, p.vec);
+        auto finish = [&](int t, const float (&g)[V]) __attribute__((always_inline)) {              // dx of input t is complete
+            if (t >= t_first && t < t_last) {
+                if (p.vec) lane_store<T, V, true>(dx + (long long)t * p.D, (unsigned)d0, g, nv);
+                else lane_store<T, V, false>(dx + (long long)t * p.D, (unsigned)d0, g, nv);
+            }
             else if (t < 0 && q == 0 && p.dstate) raw_store<T, V>((T*)p.dstate + ((long long)b * (W - 1) + t + W - 1) * p.D + d0, g, nv, p.vec);
         };
         // taps that a start before t_first cut off from the state: their rows get no gradient (they stay zero); inside the run `alive` says so
         const int stop = t_last + W - 1 < len ? t_last + W - 1 : len;           // steps walked: [t_first, stop)
         constexpr int U = 4;
-        int s = t_first;
-        for (int s0 = t_first; s0 < stop; s0 += U) {
+        // One group of U steps from s0 on.  EASY: whole vectors and no starts; OWN: steps of this run (the ones behind it give no share of dweight and
+        // dbias here); FULL: all U steps are before `to`.  All of it uniform over the wave.
+        auto group = [&](auto easy_, auto own_, auto full_, int s0, int to) __attribute__((always_inline)) {
+            constexpr bool EASY = decltype(easy_)::value, STARTS = !EASY, OWN = decltype(own_)::value, FULL = decltype(full_)::value;
             RawVec<T, V> rx[U], rg[U];
             bool st[U];
-            if (p.vec && !ps && s0 + U <= stop) {      // (uniform over the wave)
 #pragma unroll
-                for (int k = 0; k < U; ++k) {
-                    rx[k] = raw_load<T, V>(px + (long long)(s0 + k) * p.x_st, nv, true);
-                    rg[k] = raw_load<T, V>(pg + (long long)(s0 + k) * p.dy_st, nv, true);
-                    st[k] = false;
+            for (int k = 0; k < U; ++k) {
+                const bool on = FULL || s0 + k < to;
+                if constexpr (EASY) {                  // (rows behind the last one of the group read it again)
+                    const long long row = on ? s0 + k : to - 1;
+                    rx[k] = lane_load<T, V, true>(px + row * p.x_st, 0, lanes);
+                    rg[k] = lane_load<T, V, true>(pg + row * p.dy_st, 0, lanes);
+                } else {
+                    rx[k] = raw_load<T, V>(px + (long long)(s0 + k) * p.x_st + d0, on ? nv : 0, p.vec);
+                    rg[k] = raw_load<T, V>(pg + (long long)(s0 + k) * p.dy_st + d0, on ? nv : 0, p.vec);
                 }
-            } else {
-#pragma unroll
-                for (int k = 0; k < U; ++k) {
-                    const bool on = s0 + k < stop;
-                    rx[k] = raw_load<T, V>(px + (long long)(s0 + k) * p.x_st, on ? nv : 0, p.vec);
-                    rg[k] = raw_load<T, V>(pg + (long long)(s0 + k) * p.dy_st, on ? nv : 0, p.vec);
-                    st[k] = ps && on && ps[s0 + k];
-                }
+                st[k] = STARTS && ps && on && ps[s0 + k];
             }
 #pragma unroll
             for (int k = 0; k < U; ++k) {
-                s = s0 + k;
-                if (s >= stop) break;
-                if (st[k]) {
+                const int s = s0 + k;
+                if (!FULL && s >= to) break;
+                if (STARTS && st[k]) {
 #pragma unroll
                     for (int j = 0; j < W - 1; ++j) alive[j] = false;
                 }
-                const bool mine = s < t_last;
 #pragma unroll
                 for (int i = 0; i < V; ++i) {
-                    if (st[k])
+                    if (STARTS && st[k])
 #pragma unroll
                         for (int j = 0; j < W - 1; ++j) win[j][i] = 0.0f;
                     win[W - 1][i] = (float)rx[k].v[i];
@@ -272,24 +280,35 @@ __global__ __launch_bounds__(256) void conv_bwd_kernel(const ConvParams p) {
 #pragma unroll
                         for (int j = 0; j < W; ++j) pre = __builtin_fmaf(w[j][i], win[j][i], pre);
                         const float sg = sigmoidf_(pre);
-                        dpre *= sg + pre * sg * (1.0f - sg);
+                        dpre *= __builtin_fmaf(pre * sg, 1.0f - sg, sg);
                     }
 #pragma unroll
                     for (int j = 0; j < W; ++j) {
-                        if (j == W - 1 || alive[j]) acc[j][i] = __builtin_fmaf(w[j][i], dpre, acc[j][i]);
-                        dw[j][i] = mine ? __builtin_fmaf(dpre, win[j][i], dw[j][i]) : dw[j][i];
+                        if (!STARTS || j == W - 1 || alive[j]) acc[j][i] = __builtin_fmaf(w[j][i], dpre, acc[j][i]);
+                        if (OWN) dw[j][i] = __builtin_fmaf(dpre, win[j][i], dw[j][i]);
                     }
-                    db[i] += mine ? dpre : 0.0f;
+                    if (OWN) db[i] += dpre;
                 }
                 finish(s - (W - 1), acc[0]);
 #pragma unroll
                 for (int j = 0; j < W - 1; ++j) {
-                    alive[j] = j + 1 < W - 1 ? alive[j + 1] : true;
+                    if (STARTS) alive[j] = j + 1 < W - 1 ? alive[j + 1] : true;
 #pragma unroll
                     for (int i = 0; i < V; ++i) { win[j][i] = win[j + 1][i]; acc[j][i] = acc[j + 1][i]; }
                 }
             }
-        }
+        };
+        auto walk = [&](auto easy) __attribute__((always_inline)) {
+            const std::true_type yes;
+            const std::false_type no;
+            const int mid = t_last < stop ? t_last : stop;
+            int s0 = t_first;
+            for (; s0 + U <= mid; s0 += U) group(easy, yes, easy, s0, mid);
+            if (s0 < mid) group(easy, yes, no, s0, mid);
+            if (W > 1 && mid < stop) group(easy, no, no, mid, stop);
+        };
+        if (p.vec && !ps) walk(std::true_type{});
+        else walk(std::false_type{});
         // what is left in the window: inputs at - (W - 1) ... at - 1, where `at` is the step behind the last walked one
         const int at = stop > t_first ? stop : t_first;
         if (at <= len || q == 0) {
@@ -310,7 +329,7 @@ __global__ __launch_bounds__(256) void conv_bwd_kernel(const ConvParams p) {
         float none[V];
 #pragma unroll
         for (int i = 0; i < V; ++i) none[i] = 0.0f;
-        for (int t = t_first > len ? t_first : len; t < t_last; ++t) raw_store<T, V>(dx + (long long)t * p.D, none, nv, p.vec);
+        for (int t = t_first > len ? t_first : len; t < t_last; ++t) raw_store<T, V>(dx + (long long)t * p.D + d0, none, nv, p.vec);
     }
     // the four walkers' sums, in order
 #pragma unroll
@@ -351,7 +370,7 @@ __global__ __launch_bounds__(1024) void conv_finish_kernel(const float* part, in
 static int conv_check(const pcrl_conv_desc* d, const char* who) {
     if (!d) return fail(PCRL_E_ARG, "%s: null descriptor", who);
     if (d->B < 1 || d->T < 1 || d->D < 1) return fail(PCRL_E_ARG, "%s: B, T, D must be positive (%d, %d, %d)", who, d->B, d->T, d->D);
-    if (d->T > 0x7FFFFFE0) return fail(PCRL_E_ARG, "%s: T = %d", who, d->T);        // (a run's end is a 32-bit step)
+    if (d->T > 0x7FFFFFE0 || d->D >= (1 << 26)) return fail(PCRL_E_ARG, "%s: T = %d, D = %d", who, d->T, d->D);        // (32-bit steps and channels)
     if (d->W < 1 || d->W > 4) return fail(PCRL_E_ARG, "%s: W = %d taps (1 to 4)", who, d->W);
     if (!seq_dtype(d->dtype)) return fail(PCRL_E_ARG, "%s: dtype %d", who, d->dtype);
     if (!d->x || !d->weight) return fail(PCRL_E_ARG, "%s: null input", who);
@@ -388,11 +407,13 @@ static int conv_fwd(ConvParams& p, hipStream_t s) {
     PCRL_CHECK_LAUNCH("conv_fwd_kernel");
     return PCRL_OK;
 }
+// Long runs read less halo, short ones fill the chip: the longest of 32, 16, 8 steps with two waves for every SIMD.  Four walkers of 64 channel
+// vectors a workgroup, about four workgroups per CU, which leave one part of the sums each.
 static void conv_bwd_plan(const pcrl_conv_desc* d, int& run, int& nrun, int& parts) {
     const int V = kConvV;
     const long long cols = (d->D + 64 * V - 1) / (64 * V);
     run = 32;
-    while (run > 8 && cols * d->B * ((d->T + run - 1) / run) < 16LL * num_cus()) run >>= 1;
+    while (run > 8 && cols * d->B * ((d->T + run - 1) / run) < 8LL * num_cus()) run >>= 1;
     nrun = (d->T + run - 1) / run;
     const long long lines = (long long)d->B * nrun, want = 4LL * num_cus() / cols;
     long long n = (lines + 3) / 4;
