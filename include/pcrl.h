@@ -601,6 +601,7 @@ int pcrl_gather_scalars_host_f32(const float* const* src, float* const* dst, con
 /* ---- sequence operators: the recurrent core's short causal convolution and selective state space scan, and dropout ----------------------
  * Activations are PCRL_DT_F32, PCRL_DT_BF16 or PCRL_DT_F16 (one type per call), [B, T, D] with strides in elements for batch and time and
  * the channels adjacent; parameters, recurrent states of the scan and every sum are float32.  Outputs without strides are dense.
+ * The scan's step strides are 0 ... 2^26 - 1 elements (offsets inside a tile of steps are 32-bit).
  *   starts  [B][T] bytes (batch stride starts_sb) or NULL: non-zero where step t is the first of a new sequence -- nothing from before it
  *           (the incoming state included) reaches it;
  *   lengths [B] or NULL: batch row b has lengths[b] steps (clamped to 0 ... T).  Outputs and gradients behind them are 0, inputs behind them are
@@ -615,7 +616,7 @@ typedef struct pcrl_conv_desc {
     const uint8_t* starts; int64_t starts_sb;
     const int32_t* lengths;
 } pcrl_conv_desc;
-/* y [B][T][D], last_state [B][W-1][D] (either may be NULL).  last_state may be the memory of `state` only when T == 1 (the acting step). */
+/* y [B][T][D], last_state [B][W-1][D] (may be NULL).  last_state may be the memory of `state` only when T == 1 (the acting step). */
 int pcrl_short_conv_fwd(const pcrl_conv_desc* d, void* y, void* last_state, void* stream);
 int pcrl_short_conv_bwd_workspace_bytes(const pcrl_conv_desc* d, size_t* bytes);
 /* Gradients of sum(y * dy) + sum(last_state * dlast): dx [B][T][D], dweight [D][W], dbias [D] or NULL, dstate [B][W-1][D] or NULL.

@@ -8,6 +8,10 @@
 // the way back.  dB and dC are sums over channels: 16 steps x 4 states of lane values per wave.  Two steps' values are folded into one register
 // as soon as both exist (each lane keeps one and sends the other: 3 instructions for 2 values instead of 6 for each value's own tree), left per
 // channel block, and added up in a fixed order by a second launch.
+// Bound by vector instructions (at 16.8 M elements, N = 16: 96 M of a wave's, 23 a state and step, 187 us of every SIMD at 4.3 cycles each; the
+// 235 MB it cannot do without would take 44 us) at two waves per SIMD: 256 registers, the states and decays of a tile 128 of them.
+// Measured at 4 x 2048 x 2048, bf16: 80 us for the chunk summaries, 257 us for the walk, 10 us for the sums.  What was slower for the walk: LDS
+// reads one group of steps ahead (302, it spills), states of half a tile at a time (264), the next tile's loads in the middle of the walk (275).
 #include "ssm_common.h"
 
 namespace pcrl {
@@ -411,7 +415,7 @@ __global__ __launch_bounds__(256, 2) void ssm_bwd_kernel(const SsmParams) {
                 const long long at = (((long long)b * p->nchunk + chunk) * p->D + dch) * p->N + n0(k);
                 float P[RN];
 #pragma unroll
-                for (int j = 0; j < RN; ++j) P[j] = cut ? 0.0f : __builtin_amdgcn_exp2f(dt_sum * A2[k][j]);
+                for (int j = 0; j < RN; ++j) P[j] = cut ? kCut : __builtin_amdgcn_exp2f(dt_sum * A2[k][j]);
                 raw_store<float, RN>(p->sum_p + at, P, count(k), p->vec_n);
                 raw_store<float, RN>(p->sum_s + at, gc[k], count(k), p->vec_n);
             } else if (chunk == 0 && p->dstate) {
@@ -494,7 +498,8 @@ __global__ __launch_bounds__(1024) void ssm_finish_kernel(const SsmFinishParams 
 }
 
 // ---- host --------------------------------------------------------------------------------------------------------------------------------
-// Batch rows that share a workgroup (their dA sums stay in registers): as many as leave about four workgroups per CU.
+// Batch rows that share a workgroup (their dA sums stay in registers, one part of them is left per workgroup): as many as leave about four
+// workgroups per CU.  Runs cut into chunks are few rows: one each.
 static int bwd_b_step(const pcrl_ssm_desc* d, const SsmPlan& plan) {
     if (plan.nchunk > 1) return d->B;
     const long long want = 4LL * num_cus() / ((long long)d->G * plan.nblk);

@@ -14,6 +14,7 @@ namespace pcrl {
 
 constexpr int kTile = 16;              // steps per tile = lanes of a DPP row
 constexpr int kSsmMaxN = 32;
+constexpr float kCut = -1.0f;          // in the place of a chunk's product of decays (never negative)
 constexpr int kInLd = 20;              // [channel][step] tile in LDS: 16-byte reads of four steps, rows 4 banks apart
 constexpr int kInTile = 16 * kInLd;
 constexpr int kPartLd = 16 * 16 + 16;  // [state row][step][channel]: the four rows of a wave write to different banks
@@ -85,7 +86,8 @@ __device__ __forceinline__ unsigned ssm_start_bits(unsigned char mine) {
     return (unsigned)__builtin_amdgcn_readfirstlane((int)((unsigned)m & 0xFFFFu));
 }
 // v = P v + S over n chunk summaries, `step` floats apart (the bases are uniform, `off` and `nn` the lane's clamped place).  Four summaries' loads are
-// in flight at a time: the chain is one multiply-add per summary, not one trip to memory.  P == 0: a start (or nothing left) inside the chunk.
+// in flight at a time: the chain is one multiply-add per summary, not one trip to memory.  P == kCut: a start inside
+// the chunk, nothing from before gets through (a zero stays one also where the decays' product has overflowed).
 template <int RN, bool VEC>
 __device__ __forceinline__ void ssm_combine(float (&v)[RN], const float* P, const float* S, long long step, int n, unsigned off, const unsigned (&nn)[RN]) {
     for (int c = 0; c < n; c += 4) {
@@ -100,7 +102,7 @@ __device__ __forceinline__ void ssm_combine(float (&v)[RN], const float* P, cons
         for (int i = 0; i < 4; ++i) {
             if (c + i < n) {
 #pragma unroll
-                for (int j = 0; j < RN; ++j) v[j] = a[i].v[j] == 0.0f ? s[i].v[j] : __builtin_fmaf(a[i].v[j], v[j], s[i].v[j]);
+                for (int j = 0; j < RN; ++j) v[j] = a[i].v[j] < 0.0f || v[j] == 0.0f ? s[i].v[j] : __builtin_fmaf(a[i].v[j], v[j], s[i].v[j]);
             }
         }
     }

@@ -1,4 +1,8 @@
 // Selective state space scan, forward and single step (ssm_common.h: the split; include/pcrl.h: the formulas).
+//
+// The walk is bound by vector instructions: per state and step an exponential, two multiplies and two multiply-adds (its bytes alone would take
+// 25 us at 16.8 M elements, N = 16, bf16).  Measured there (4 x 2048 x 2048): 64 us for the chunk summaries and 93 us for the walk, whose 33.3 M
+// wave instructions (8 a state and step) are 65 us of every SIMD at 4.3 cycles each; 1 x 16384 x 1024: 62 and 111 us.
 #include "ssm_common.h"
 
 namespace pcrl {
@@ -195,7 +199,7 @@ __global__ __launch_bounds__(256) void ssm_fwd_kernel(const SsmParams) {
             const long long at = (((long long)b * p->nchunk + chunk) * p->D + dch) * p->N + n0(k);
             float P[RN];
 #pragma unroll
-            for (int j = 0; j < RN; ++j) P[j] = cut ? 0.0f : __builtin_amdgcn_exp2f(dt_sum * A2[k][j]);
+            for (int j = 0; j < RN; ++j) P[j] = cut ? kCut : __builtin_amdgcn_exp2f(dt_sum * A2[k][j]);
             raw_store<float, RN>(p->sum_p + at, P, count(k), p->vec_n);
             raw_store<float, RN>(p->sum_s + at, h[k], count(k), p->vec_n);
         } else if (p->last && chunk == p->nchunk - 1) {
@@ -206,7 +210,8 @@ __global__ __launch_bounds__(256) void ssm_fwd_kernel(const SsmParams) {
 
 // One step.  The state is 8 N bytes per channel of traffic against a few of everything else, so lanes run along it: LPC lanes per channel, four
 // states each (16-byte accesses when N % 4 == 0), the sum over the states inside the group of LPC lanes.  A workgroup keeps its A and walks
-// batch rows b, b + b_step, ..., the next row's loads in flight while this one is computed.
+// batch rows b, b + b_step, ..., the next row's loads in flight while this one is computed.  Bound by memory: 1024 x 1024 channels, N = 16, bf16
+// (134 MB of states) take 24.4 us = 5.5 TB/s, the rate of a large copy; one row of 256 channels 2.7 us, a launch.
 struct SsmStepParams {
     SsmParams s;
     float* state_out;
@@ -319,7 +324,7 @@ void ssm_fill(SsmParams& p, const pcrl_ssm_desc* d) {
 // (0.4 to 0.7 of the forward's walk, 0.2 to 0.3 of the backward's).  Measured on 16.8 M elements, bf16, N = 16, us (forward / backward, all launches) at 1, 2, 4, 8
 // chunks: 128 blocks 321 / 818, 262 / 492, 174 / 343, 152 / 335; 256 blocks 162 / 376, 154 / 329, 140 / 327, -; 384 blocks (25 M elements) 189 / 496,
 // 208 / 498, 208 / 482, -; 512 blocks 104 / 268, 126 / 307, 139 / 333, -.  So: none from 1.5 blocks per CU on, else up to 4 workgroups per CU forward
-// and 2 backward (its registers and LDS admit no more), down to single tiles (a 333-step batch of 28 blocks: 21 chunks 19 / 33, 7 chunks 21 / 38).
+// and 2 backward (its registers and LDS admit no more), down to single tiles (333 steps, 28 blocks: 21 chunks 19 / 33, 11 chunks 21 / 37, 7 chunks 21 / 38).
 SsmPlan ssm_plan(const pcrl_ssm_desc* d, bool backward) {
     SsmPlan plan{};
     const int ntile = cdiv(d->T, kTile);
@@ -416,7 +421,7 @@ extern "C" int pcrl_ssm_step(const pcrl_ssm_desc* d, void* y, float* state_out, 
     if (width > 0x7FFFFFFFLL) return fail(PCRL_E_ARG, "pcrl_ssm_step: D = %d", d->D);
     q.rows = width < 256 ? (int)(256 / width) : 1;
     const unsigned gx = q.rows > 1 ? 1u : (unsigned)cdiv(width, 256), groups = (unsigned)cdiv(d->B, q.rows);
-    // workgroups for every row, up to about eight per CU; beyond that each walks several rows
+    // workgroups for every row, up to about eight per CU (all resident at once); beyond that each walks several rows
     unsigned gy = (unsigned)((8LL * num_cus() + gx - 1) / gx);
     gy = gy < 1 ? 1 : gy > 65535 ? 65535 : gy;
     gy = gy < groups ? gy : groups;

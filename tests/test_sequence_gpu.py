@@ -578,6 +578,116 @@ def test_the_c_entry_points_refuse_bad_descriptors():
         assert drop(*args) == -1, args
 
 
+@pytest.mark.gpu
+def test_a_zero_state_stays_zero_where_the_decays_overflow(cuda):
+    """Growing states (A > 0), chunks whose product of decays is beyond float32: what is zero in front of such a chunk is zero behind it, both ways."""
+    kw, on, dy, dlast = scan_inputs(cuda, F32, 1, 1500, 64, 16, z=False, skip=False, bias=False, state=False)
+    kw["A"] = torch.full_like(kw["A"], 8.0)                    # e^8 a step, e^128 over a tile of 16
+    kw["dt"] = torch.ones_like(kw["dt"])
+    kw["u"][:, :-3] = 0.0
+    dy[:, 2:] = 0.0
+    on.update((n, kw[n].to(cuda)) for n in ("A", "dt", "u"))
+    check_scan(cuda, kw, on, dy, torch.zeros_like(dlast), softplus=False)
+
+
+@pytest.mark.gpu
+def test_lengths_of_64_bits(cuda):
+    from pointcloud_rl_amd import sequence
+    kw, on, _, _ = scan_inputs(cuda, F32, 3, 20, 24, 8)
+    wide = torch.tensor([2 ** 40 + 3, -2 ** 40, 7], device=cuda)
+    narrow = torch.tensor([20, 0, 7], dtype=torch.int32, device=cuda)
+    for a, b in zip(sequence.ssm_scan(**on, lengths=wide), sequence.ssm_scan(**on, lengths=narrow)):
+        assert torch.equal(a, b)
+    w = torch.randn(24, 4, device=cuda)
+    for a, b in zip(sequence.short_conv(on["u"], w, lengths=wide), sequence.short_conv(on["u"], w, lengths=narrow)):
+        assert torch.equal(a, b)
+
+
+@pytest.mark.gpu
+def test_steps_far_apart_in_memory(cuda):
+    """A step stride beyond what the scan's offsets reach: the input is copied."""
+    from pointcloud_rl_amd import sequence
+    base = torch.zeros((1 << 26) + 64, dtype=BF16, device=cuda)
+    kw, on, _, _ = scan_inputs(cuda, BF16, 1, 2, 16, 4)
+    far = base.as_strided((1, 2, 16), (1 << 27, 1 << 26, 1))
+    far.copy_(on["u"])
+    want = sequence.ssm_scan(**on)
+    for a, b in zip(sequence.ssm_scan(**dict(on, u=far)), want):
+        assert torch.equal(a, b)
+    w = torch.randn(16, 4, device=cuda)
+    for a, b in zip(sequence.short_conv(far, w), sequence.short_conv(on["u"], w)):
+        assert torch.equal(a, b)
+
+
+@pytest.mark.gpu
+def test_second_derivatives_are_refused(cuda):
+    from pointcloud_rl_amd import sequence
+    kw, on, _, _ = scan_inputs(cuda, F32, 1, 5, 8, 4)
+    u = on["u"].requires_grad_()
+    for y in (sequence.ssm_scan(**on)[0], sequence.short_conv(u, torch.randn(8, 4, device=cuda))[0], sequence.dropout(u, 0.5, 3)):
+        with pytest.raises(RuntimeError, match="differentiable once"):
+            torch.autograd.grad(y.sum(), u, create_graph=True)
+
+
+@pytest.mark.gpu
+def test_a_state_updated_in_place_does_not_pass_for_the_saved_one(cuda):
+    from pointcloud_rl_amd import sequence
+    kw, on, _, _ = scan_inputs(cuda, F32, 2, 5, 8, 4)
+    y, _ = sequence.ssm_scan(**dict(on, u=on["u"].requires_grad_()))
+    step = {n: on[n][:, 0] if n in ("u", "dt", "B", "C", "z") else on[n] for n in on}
+    sequence.ssm_step(**step)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.sum().backward()
+    conv = torch.zeros(2, 3, 8, device=cuda)
+    w = torch.randn(8, 4, device=cuda, requires_grad=True)
+    y, _ = sequence.short_conv(on["u"].detach(), w, state=conv)
+    sequence.short_conv_step(on["u"][:, 0].detach(), conv, w)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.sum().backward()
+
+
+@pytest.mark.gpu
+def test_steps_in_inference_mode(cuda):
+    from pointcloud_rl_amd import sequence
+    x, w = torch.randn(2, 8, device=cuda), torch.randn(8, 4, device=cuda)
+    outer = torch.zeros(2, 3, 8, device=cuda)
+    want = sequence.short_conv_step(x, outer.clone(), w)
+    with torch.inference_mode():
+        inner = torch.zeros(2, 3, 8, device=cuda)
+        assert torch.equal(sequence.short_conv_step(x, inner, w), want) and torch.equal(sequence.short_conv_step(x, outer, w), want)
+        assert torch.equal(inner, outer)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n", [1, 7, 4099])
+def test_dropout_in_place_through_the_c_entry_point(cuda, n):
+    from pointcloud_rl_amd import _lib, sequence
+    x, r = torch.randn(n, device=cuda), torch.randn(n, device=cuda)
+    want = sequence.dropout(x, 0.25, 11, offset=5, residual=r)
+    at = lambda t: ctypes.c_void_p(t.data_ptr())
+    stream = ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)
+    ld, one, seed, offset = ctypes.c_int64(n), ctypes.c_int64(1), ctypes.c_uint64(11), ctypes.c_uint64(5)
+    for out in (x.clone(), r.clone()):
+        a, b = (out, r) if torch.equal(out, x) else (x, out)
+        assert _lib.lib().pcrl_dropout(at(a), ld, at(b), ld, at(out), one, ld, 0, 1 << 14, seed, offset, None, stream) == 0
+        assert torch.equal(out, want)
+
+
+def test_sizes_beyond_the_kernels_indexes_are_refused():
+    from pointcloud_rl_amd import _lib
+    lib = _lib.lib()
+    one, n = ctypes.c_void_p(4096), ctypes.c_size_t()      # never dereferenced
+    for kw in (dict(T=0x7FFFFFF0), dict(B=(1 << 30) + 1), dict(D=1 << 26), dict(u_st=1 << 26), dict(dt_st=-1), dict(c_st=1 << 26)):
+        d = SsmDesc(**dict(dict(B=1, T=2, D=8, N=4, G=1, u=4096, dt=4096, Bm=4096, Cm=4096, A=4096), **kw))
+        assert lib.pcrl_ssm_scan_fwd(ctypes.byref(d), one, None, None, None, ctypes.c_size_t(0), None) == -1, kw
+        assert lib.pcrl_ssm_scan_bytes(ctypes.byref(d), ctypes.byref(n), None, None) == -1, kw
+    for kw in (dict(T=0x7FFFFFF0), dict(D=1 << 26), dict(B=1 << 24, T=1 << 12, D=64)):
+        d = ConvDesc(**dict(dict(B=1, T=2, D=8, W=4, x=4096, weight=4096), **kw))
+        assert lib.pcrl_short_conv_fwd(ctypes.byref(d), one, None, None) == -1, kw
+    big = ctypes.c_int64(1 << 36)
+    assert lib.pcrl_dropout(one, big, None, big, one, ctypes.c_int64(1), big, 0, 1, ctypes.c_uint64(0), ctypes.c_uint64(0), None, None) == -1
+
+
 def test_struct_layouts_match_the_header(tmp_path):
     """sizeof / offsetof of the sequence descriptors as gcc lays them out == the ctypes mirror."""
     import os
