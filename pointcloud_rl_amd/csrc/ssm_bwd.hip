@@ -94,7 +94,7 @@ __global__ __launch_bounds__(256, 2) void ssm_bwd_kernel(const SsmParams) {
     float* s_gb = s_slope + 256;                        // [state row][step][channel]: sum_n g B
     float* s_aw = s_gb + kPartTile;                     // ... sum_n A w
     float* s_y = s_aw + kPartTile;                      // ... sum_n C h
-    float* s_bc = lds + 4 * kWave;                      // [4 waves][dB, dC][16 steps][states]: the four waves' sums over their channels
+    float* s_bc = lds + 4 * kWave;                      // [4 waves][dB, dC][16 steps][states of a group]: the four waves' sums over their channels
     int blk, chunk, b0;
     ssm_where(p, blk, chunk, b0);
     if (SUMMARY && chunk == 0) return;                  // nobody ends at the first chunk's summary
@@ -164,10 +164,21 @@ __global__ __launch_bounds__(256, 2) void ssm_bwd_kernel(const SsmParams) {
         bool cut = false;
 
         RawVec<T, 4> nu, nd, nz, ng;
-        RawVec<T, RN> nB[NG], nC[NG];
-        RawVec<float, RN> nh[NG];
+        // State groups in flight: all, or (the walk) the next one it comes to; dB and dC leave LDS by the group as well, so that two workgroups fit
+        // a CU with two groups too.  N = 32 at 4 x 2048 x 2048: 811 us with both held, 710 with LDS for one, 543 with registers for one.
+        constexpr int NF = SUMMARY ? NG : 1;
+        RawVec<T, RN> nB[NF], nC[NF];
+        RawVec<float, RN> nh[NF];
         unsigned nst = 0;
-        auto fetch = [&](int tile) {                    // rows behind the length read the last one
+        auto fetch_states = [&](int tile, int k, int to) {          // rows behind the length read the last one, here and below
+            const SsmArgs p = ssm_args();
+            const long long t0 = (long long)tile * kTile;
+            const int last = len - 1 - (int)t0, rn = ch < last ? ch : last;
+            if (!SUMMARY) nB[to] = lane_load<T, RN, VEC>(pB + t0 * p->b_st, rn * (unsigned)p->b_st, nn[k]);
+            nC[to] = lane_load<T, RN, VEC>(pC + t0 * p->c_st, rn * (unsigned)p->c_st, nn[k]);
+            if (!SUMMARY) nh[to] = lane_load<float, RN, VEC>(p->saved + (((long long)b * p->ntile + tile) * p->D + d_first) * p->N, o_h, nn[k]);
+        };
+        auto fetch = [&](int tile) {
             const SsmArgs p = ssm_args();
             const long long t0 = (long long)tile * kTile;
             const int last = len - 1 - (int)t0, r = row < last ? row : last, rn = ch < last ? ch : last;
@@ -176,11 +187,7 @@ __global__ __launch_bounds__(256, 2) void ssm_bwd_kernel(const SsmParams) {
             if (pz) nz = lane_load<T, 4, VEC>(pz + t0 * p->z_st, r * (unsigned)p->z_st, cc);
             ng = lane_load<T, 4, VEC>(pg + t0 * p->dy_st, r * (unsigned)p->dy_st, cc);
 #pragma unroll
-            for (int k = 0; k < NG; ++k) {
-                if (!SUMMARY) nB[k] = lane_load<T, RN, VEC>(pB + t0 * p->b_st, rn * (unsigned)p->b_st, nn[k]);
-                nC[k] = lane_load<T, RN, VEC>(pC + t0 * p->c_st, rn * (unsigned)p->c_st, nn[k]);
-                if (!SUMMARY) nh[k] = lane_load<float, RN, VEC>(p->saved + (((long long)b * p->ntile + tile) * p->D + d_first) * p->N, o_h, nn[k]);
-            }
+            for (int k = 0; k < NF; ++k) fetch_states(tile, k, k);
             if (ps) nst = ch <= last ? ps[t0 + rn] : 0;
         };
         const int live = (len + kTile - 1) / kTile, end = tile1 < live ? tile1 : live;
@@ -202,14 +209,25 @@ __global__ __launch_bounds__(256, 2) void ssm_bwd_kernel(const SsmParams) {
             const bool plain = clean && t0 + kTile <= len, here = t0 + row < len;
             RawVec<T, 4> ru = nu, rz = nz, rg = ng;     // kept as they came: half the registers of a 16-bit type
             float Bv[NG][RN], Cv[NG][RN], h0[NG][RN];
-#pragma unroll
-            for (int k = 0; k < NG; ++k)
+            auto states = [&](int k, int from) __attribute__((always_inline)) {
 #pragma unroll
                 for (int j = 0; j < RN; ++j) {
-                    Bv[k][j] = !SUMMARY ? (float)nB[k].v[j] : 0.0f;
-                    Cv[k][j] = (float)nC[k].v[j];
-                    h0[k][j] = !SUMMARY ? nh[k].v[j] : 0.0f;
+                    Bv[k][j] = !SUMMARY ? (float)nB[from].v[j] : 0.0f;
+                    Cv[k][j] = (float)nC[from].v[j];
+                    h0[k][j] = !SUMMARY ? nh[from].v[j] : 0.0f;
                 }
+                if (!plain) {
+#pragma unroll
+                    for (int j = 0; j < RN; ++j) {
+                        const bool on = t0 + ch < len && n0(k) + j < p->N;
+                        Bv[k][j] = on ? Bv[k][j] : 0.0f;
+                        Cv[k][j] = on ? Cv[k][j] : 0.0f;
+                        h0[k][j] = j < count(k) ? h0[k][j] : 0.0f;
+                    }
+                }
+            };
+#pragma unroll
+            for (int k = 0; k < NF; ++k) states(k, k);
             if (!plain) {                               // what does not exist counts for nothing (also in the sums over the channels)
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
@@ -218,15 +236,6 @@ __global__ __launch_bounds__(256, 2) void ssm_bwd_kernel(const SsmParams) {
                     rz.v[i] = on && pz ? rz.v[i] : (T)0.0f;
                     rg.v[i] = on ? rg.v[i] : (T)0.0f;
                 }
-#pragma unroll
-                for (int k = 0; k < NG; ++k)
-#pragma unroll
-                    for (int j = 0; j < RN; ++j) {
-                        const bool on = t0 + ch < len && n0(k) + j < p->N;
-                        Bv[k][j] = on ? Bv[k][j] : 0.0f;
-                        Cv[k][j] = on ? Cv[k][j] : 0.0f;
-                        h0[k][j] = j < count(k) ? h0[k][j] : 0.0f;
-                    }
             }
             {
                 const f32x4 bias = *(const f32x4*)(s_bias + c0);
@@ -262,7 +271,19 @@ __global__ __launch_bounds__(256, 2) void ssm_bwd_kernel(const SsmParams) {
             const unsigned starts = ps ? ssm_start_bits(nst) : 0u;
             if constexpr (SUMMARY) wave_lds_fence();
             else __syncthreads();                       // the last tile's s_bc has been read
-            if (tile > tile0) fetch(tile - 1);
+            if (NF < NG) fetch_states(tile, 1, 0);
+            else if (tile > tile0) fetch(tile - 1);
+            // dB and dC of the tile and of state group k over the workgroup's 64 channels
+            constexpr int W = 4 * RN;                   // states of a group as they stand in LDS (N of all exist)
+            auto add_bc = [&](int k) __attribute__((always_inline)) {
+                const SsmArgs p = ssm_args();
+                for (int e = threadIdx.x; e < 2 * 16 * W; e += 256) {
+                    const float* src = s_bc + e;
+                    const float v = (src[0] + src[2 * 16 * W]) + (src[2 * 2 * 16 * W] + src[3 * 2 * 16 * W]);
+                    const int which = e / (16 * W), t = (e / W) % 16, n_ = k * W + e % W;
+                    if (n_ < p->N && t0 + t < len) (which ? p->part_c : p->part_b)[(((long long)blk * p->B + b) * p->T + t0 + t) * p->N + n_] = v;
+                }
+            };
             auto walk = [&](auto with_starts) {
                 constexpr bool WS = decltype(with_starts)::value;
                 if constexpr (SUMMARY) {
@@ -287,6 +308,11 @@ __global__ __launch_bounds__(256, 2) void ssm_bwd_kernel(const SsmParams) {
                 } else {
                     static_for<NG>([&](auto kc) {
                         constexpr int k = decltype(kc)::value;
+                        if (k > 0) {
+                            states(k, 0);
+                            if (k + 1 < NG) fetch_states(tile, k + 1, 0);
+                            else if (tile > tile0) fetch(tile - 1);
+                        }
                         float a[kTile][RN], h[kTile][RN];
                         static_for<4>([&](auto gi) {
                             constexpr int tg = decltype(gi)::value * 4;
@@ -338,13 +364,18 @@ __global__ __launch_bounds__(256, 2) void ssm_bwd_kernel(const SsmParams) {
                             });
                         });
                         // this wave's sums over its channels, [step][state]: lane (q, ch) has step folded_step(ch), states n0(k) ...
-                        float* out = s_bc + wave * (2 * 16 * 4 * RN * NG) + folded_step(ch) * (4 * RN * NG) + n0(k);
+                        float* out = s_bc + wave * (2 * 16 * W) + folded_step(ch) * W + q * RN;
                         if constexpr (RN == 4) {
                             *(f32x4*)out = f32x4{hb[3][0], hb[3][1], hb[3][2], hb[3][3]};
-                            *(f32x4*)(out + 16 * 4 * RN * NG) = f32x4{hc[3][0], hc[3][1], hc[3][2], hc[3][3]};
+                            *(f32x4*)(out + 16 * W) = f32x4{hc[3][0], hc[3][1], hc[3][2], hc[3][3]};
                         } else {
 #pragma unroll
-                            for (int j = 0; j < RN; ++j) { out[j] = hb[3][j]; out[16 * 4 * RN * NG + j] = hc[3][j]; }
+                            for (int j = 0; j < RN; ++j) { out[j] = hb[3][j]; out[16 * W + j] = hc[3][j]; }
+                        }
+                        if constexpr (k + 1 < NG) {
+                            __syncthreads();
+                            add_bc(k);
+                            __syncthreads();            // before the next group's
                         }
                     });
                 }
@@ -398,15 +429,8 @@ __global__ __launch_bounds__(256, 2) void ssm_bwd_kernel(const SsmParams) {
                 lane_store<T, 4, VEC>((T*)p->du + to, o, o_u, n);
                 lane_store<T, 4, VEC>((T*)p->ddt + to, o, o_dt, n);
                 if (pz) lane_store<T, 4, VEC>((T*)p->dz + to, o, o_z, n);
-                // dB and dC of the tile over the workgroup's 64 channels
                 __syncthreads();
-                constexpr int W = 4 * RN * NG;          // states as they stand in LDS (N of them exist)
-                for (int e = threadIdx.x; e < 2 * 16 * W; e += 256) {
-                    const float* src = s_bc + e;
-                    const float v = (src[0] + src[2 * 16 * W]) + (src[2 * 2 * 16 * W] + src[3 * 2 * 16 * W]);
-                    const int which = e / (16 * W), t = (e / W) % 16, n_ = e % W;
-                    if (n_ < p->N && t0 + t < len) (which ? p->part_c : p->part_b)[(((long long)blk * p->B + b) * p->T + t0 + t) * p->N + n_] = v;
-                }
+                add_bc(NG - 1);
             }
         }
 #pragma unroll
@@ -528,7 +552,7 @@ static int launch_bwd(const SsmParams& p, hipStream_t s) {
         ssm_bwd_kernel<T, RN, NG, VEC, true><<<grid, 256, sizeof(float) * 4 * ssm_bwd_wave_lds<true>(), s>>>(p);
         PCRL_CHECK_LAUNCH("ssm_bwd_kernel (summary)");
     }
-    const size_t lds = sizeof(float) * (4 * ssm_bwd_wave_lds<false>() + 4 * 2 * 16 * 4 * RN * NG);
+    const size_t lds = sizeof(float) * (4 * ssm_bwd_wave_lds<false>() + 4 * 2 * 16 * 4 * RN);
     if (int rc = ensure_dynamic_lds((const void*)ssm_bwd_kernel<T, RN, NG, VEC, false>, lds)) return rc;
     ssm_bwd_kernel<T, RN, NG, VEC, false><<<grid, 256, lds, s>>>(p);
     PCRL_CHECK_LAUNCH("ssm_bwd_kernel");
