@@ -360,13 +360,20 @@ Tensor ssm_step(const Tensor& u, const Tensor& dt, const Tensor& A, const Tensor
 }
 
 // ---- dropout ---------------------------------------------------------------------------------------------------------------------------------
-// t as rows x cols with adjacent columns; what cannot be seen that way is copied.
+// t as rows x cols with adjacent columns; what cannot be seen that way is copied.  An axis of one element takes no part: its stride is never
+// stepped over and may be anything.
 struct Rows { Tensor t; int64_t rows, cols, ld; };
 Rows rows_of(const Tensor& t) {
     if (!t.is_contiguous() && t.stride(-1) == 1) {
-        bool flat = true;                                       // the leading dimensions collapse into one with a single stride
-        for (int64_t i = 0; i + 2 < t.dim(); ++i) flat = flat && (t.size(i) == 1 || t.stride(i) == t.stride(i + 1) * t.size(i + 1));
-        if (flat && t.stride(-2) >= 0) return {t, t.numel() / t.size(-1), t.size(-1), t.stride(-2)};
+        int64_t rows = 1, ld = t.size(-1);
+        bool flat = true;                                       // the leading axes collapse into one with a single stride
+        for (int64_t i = t.dim() - 2; i >= 0 && flat; --i) {
+            if (t.size(i) == 1) continue;
+            if (rows == 1) ld = t.stride(i);
+            else flat = t.stride(i) == ld * rows;
+            rows *= t.size(i);
+        }
+        if (flat && ld >= 0) return {t, rows, t.size(-1), ld};
     }
     const Tensor c = t.contiguous();
     return {c, 1, c.numel(), c.numel()};
@@ -434,4 +441,9 @@ PYBIND11_MODULE(_sequence, m) {
     m.def("ssm_scan", &ssm_scan);
     m.def("ssm_step", &ssm_step);
     m.def("dropout", &dropout);
+    // how dropout walks a tensor (tests): rows, columns, row stride, whether it works on a copy
+    m.def("dropout_rows", [](const Tensor& t) {
+        const Rows r = rows_of(t);
+        return std::make_tuple(r.rows, r.cols, r.ld, !r.t.is_same(t));
+    });
 }
