@@ -100,6 +100,8 @@ Tensor lengths_of(const Opt& lengths, int64_t rows, int64_t steps, const Tensor&
                       "lengths is ", lengths->scalar_type(), " ", lengths->sizes(), " on ", lengths->device(), ", expected int32 [", rows, "] on ", like.device());
     return lengths->scalar_type() == at::kInt ? lengths->contiguous() : lengths->clamp(0, steps).to(at::kInt);
 }
+// Stride between steps; 0 where there is only one (a view's stride over an axis of one element may be anything).
+int64_t step_stride(const Tensor& t) { return t.size(1) == 1 ? 0 : t.stride(1); }
 bool wants_grad(std::initializer_list<Tensor> ts) {
     if (!at::GradMode::is_enabled()) return false;
     for (const Tensor& t : ts) if (t.defined() && t.requires_grad()) return true;
@@ -123,7 +125,7 @@ pcrl_conv_desc conv_desc(const Tensor& x, const Tensor& weight, const Tensor& bi
     const bool step = x.dim() == 2;
     d.B = fits("batch", x.size(0)), d.T = step ? 1 : fits("steps", x.size(1)), d.D = fits("channels", x.size(-1)), d.W = (int)weight.size(1);
     d.dtype = dtype_code(x), d.silu = silu;
-    d.x = at_(x), d.x_sb = x.stride(0), d.x_st = step ? 0 : x.stride(1);
+    d.x = at_(x), d.x_sb = x.stride(0), d.x_st = step ? 0 : step_stride(x);
     d.weight = fat(weight), d.bias = fat(bias), d.state = at_(state);
     d.starts = (const uint8_t*)at_(starts), d.starts_sb = d.T, d.lengths = (const int32_t*)at_(lengths);
     return d;
@@ -161,7 +163,7 @@ struct ConvNode : Function<ConvNode> {
             size_t need = 0;
             check(api.conv_bwd_bytes(&d, &need));
             const Tensor work = at::empty({(int64_t)need}, dx.options().dtype(at::kByte));
-            check(api.conv_bwd(&d, at_(dy), dy.stride(0), dy.stride(1), at_(dlast), to_(dx), (float*)to_(dweight), (float*)to_(dbias), to_(dstate), to_(work), need, on.stream));
+            check(api.conv_bwd(&d, at_(dy), dy.stride(0), step_stride(dy), at_(dlast), to_(dx), (float*)to_(dweight), (float*)to_(dbias), to_(dstate), to_(work), need, on.stream));
         } else {                                                // no step: the state passes through
             dweight.zero_();
             if (dbias.defined()) dbias.zero_();
@@ -235,7 +237,7 @@ pcrl_ssm_desc scan_desc(const ScanArgs& a) {
     const bool step = a.u.dim() == 2;
     d.B = fits("batch", a.u.size(0)), d.T = step ? 1 : fits("steps", a.u.size(1)), d.D = fits("channels", a.u.size(-1)), d.N = (int)a.A.size(1);
     d.G = fits("groups", a.B.size(-2)), d.dtype = dtype_code(a.u), d.softplus = a.softplus;
-    auto st = [&](const Tensor& t) { return step ? 0 : t.stride(1); };
+    auto st = [&](const Tensor& t) { return step ? 0 : step_stride(t); };
     d.u = at_(a.u), d.dt = at_(a.dt), d.z = at_(a.z), d.Bm = at_(a.B), d.Cm = at_(a.C);
     d.u_sb = a.u.stride(0), d.u_st = st(a.u), d.dt_sb = a.dt.stride(0), d.dt_st = st(a.dt);
     if (a.z.defined()) d.z_sb = a.z.stride(0), d.z_st = st(a.z);
@@ -295,7 +297,7 @@ struct ScanNode : Function<ScanNode> {
             pcrl_ssm_grads o{};
             o.du = to_(g[0]), o.ddt = to_(g[1]), o.dz = to_(g[6]), o.dB = to_(g[3]), o.dC = to_(g[4]);
             o.dA = (float*)to_(g[2]), o.dD = (float*)to_(g[5]), o.ddt_bias = (float*)to_(g[7]), o.dstate = (float*)to_(g[8]);
-            check(api.scan_bwd(&d, fat(s[11]), at_(dy), dy.stride(0), dy.stride(1), fat(dlast), &o, to_(work), (size_t)bytes, on.stream));
+            check(api.scan_bwd(&d, fat(s[11]), at_(dy), dy.stride(0), step_stride(dy), fat(dlast), &o, to_(work), (size_t)bytes, on.stream));
         } else {                                                // no step: the state passes through
             for (int i = 0; i < 8; ++i) if (g[i].defined()) g[i].zero_();
             if (g[8].defined()) { if (dlast.defined()) g[8].copy_(dlast); else g[8].zero_(); }

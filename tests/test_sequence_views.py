@@ -85,3 +85,27 @@ def test_dropout_of_views_equals_dropout_of_their_copies(cuda, dtype):
         by_view, = torch.autograd.grad(y, x, v, retain_graph=True)
         by_copy, = torch.autograd.grad(y, x, dense)
         assert torch.equal(by_view, by_copy), name
+
+
+@pytest.mark.gpu
+def test_the_stride_of_a_single_step_may_be_anything(cuda):
+    """[B, 1, D] views whose step axis has a stride beyond the scan's 32-bit offsets, which nothing steps over: the contiguous call's bits."""
+    from pointcloud_rl_amd import sequence
+    B, D, N = 2, 16, 4
+    g = torch.Generator().manual_seed(2)
+    r = lambda *s: torch.randn(*s, generator=g).to(cuda)
+    dense = dict(u=r(B, 1, D), dt=r(B, 1, D), z=r(B, 1, D), B=r(B, 1, 1, N), C=r(B, 1, 1, N))
+    rest = dict(A=-r(D, N).abs(), D=r(D), dt_bias=r(D), state=r(B, D, N))
+    far = lambda t: t.as_strided(t.shape, (t.stride(0), 1 << 27) + t.stride()[2:])
+    dy, w = r(B, 1, D), r(D, 4)
+
+    def passes(view):
+        leaves = {k: v.clone().requires_grad_() for k, v in dense.items()}
+        seen = {k: view(v) for k, v in leaves.items()}
+        y, last = sequence.ssm_scan(**seen, **rest)
+        x = dense["u"].clone().requires_grad_()
+        c, clast = sequence.short_conv(view(x), w)
+        return [y, last, c, clast] + list(torch.autograd.grad(y, list(leaves.values()), view(dy))) + list(torch.autograd.grad(c, x, view(dy)))
+
+    for i, (a, b) in enumerate(zip(passes(far), passes(lambda t: t))):
+        assert torch.equal(a, b), i
