@@ -107,6 +107,11 @@ bool wants_grad(std::initializer_list<Tensor> ts) {
     for (const Tensor& t : ts) if (t.defined() && t.requires_grad()) return true;
     return false;
 }
+// The kernels carry no tangents: a forward-mode derivative through them would come out as zero.
+void no_tangents(std::initializer_list<Tensor> ts) {
+    for (const Tensor& t : ts)
+        TORCH_CHECK_NOT_IMPLEMENTED(!t.defined() || !t._fw_grad(/*level=*/0).defined(), "the sequence operators have no forward-mode derivatives (an input is a dual tensor)");
+}
 // The gradient of an output that may take no part in the loss: zeros that are one row in memory.
 Tensor full_grad(const Tensor& g, const Tensor& like) {
     if (!g.defined()) return at::zeros({like.size(-1)}, like.options()).expand(like.sizes());
@@ -207,6 +212,7 @@ void written(const Tensor& t) { if (!t.is_inference()) t.unsafeGetTensorImpl()->
 std::tuple<Tensor, Tensor> short_conv(const Tensor& x, const Tensor& weight, const Opt& bias, const Opt& state, const Opt& starts, const Opt& lengths,
                                       const std::optional<std::string>& act) {
     ConvArgs a = conv_args(x, weight, bias, state, starts, lengths, act, 3);
+    no_tangents({a.x, a.weight, a.bias, a.state});
     on_gpu(x);
     if (a.state.defined()) a.state = a.state.contiguous();
     const variable_list r = wants_grad({a.x, a.weight, a.bias, a.state}) ? ConvNode::apply(a.x, a.weight, opt(a.bias), opt(a.state), opt(a.starts), opt(a.lengths), a.silu)
@@ -217,6 +223,7 @@ Tensor short_conv_step(const Tensor& x, const Opt& state, const Tensor& weight, 
     at::NoGradGuard no_grad;
     TORCH_CHECK_VALUE(state.has_value(), "a step needs a state");
     const ConvArgs a = conv_args(x, weight, bias, state, starts, std::nullopt, act, 2);
+    no_tangents({a.x, a.weight, a.bias, a.state});
     const Tensor out = state_out_of(a.state, state_out);
     on_gpu(x);
     Tensor y = at::empty(x.sizes(), x.options().requires_grad(false));
@@ -337,6 +344,7 @@ ScanArgs scan_args(const Tensor& u, const Tensor& dt, const Tensor& A, const Ten
 std::tuple<Tensor, Tensor> ssm_scan(const Tensor& u, const Tensor& dt, const Tensor& A, const Tensor& B, const Tensor& C, const Opt& D, const Opt& z, const Opt& dt_bias,
                                     bool softplus, const Opt& state, const Opt& starts, const Opt& lengths) {
     const ScanArgs a = scan_args(u, dt, A, B, C, D, z, dt_bias, softplus, state, starts, lengths, 3);
+    no_tangents({a.u, a.dt, a.A, a.B, a.C, a.D, a.z, a.dt_bias, a.state});
     on_gpu(u);
     int64_t bytes = 0;
     const variable_list r = wants_grad({a.u, a.dt, a.A, a.B, a.C, a.D, a.z, a.dt_bias, a.state})
@@ -349,6 +357,7 @@ Tensor ssm_step(const Tensor& u, const Tensor& dt, const Tensor& A, const Tensor
     at::NoGradGuard no_grad;
     TORCH_CHECK_VALUE(state.has_value(), "a step needs a state");
     const ScanArgs a = scan_args(u, dt, A, B, C, D, z, dt_bias, softplus, state, starts, std::nullopt, 2);
+    no_tangents({a.u, a.dt, a.A, a.B, a.C, a.D, a.z, a.dt_bias, a.state});
     const Tensor out = state_out_of(a.state, state_out);
     on_gpu(u);
     Tensor y = at::empty(u.sizes(), u.options().requires_grad(false));
@@ -428,6 +437,7 @@ Tensor dropout(const Tensor& x, double p, uint64_t seed, uint64_t offset, const 
     if (offset_t.defined())
         TORCH_CHECK_VALUE(offset_t.scalar_type() == at::kLong && offset_t.numel() == 1 && offset_t.device() == x.device(),
                           "offset: an integer, or an int64 tensor of one element on the device of x");
+    no_tangents({x, residual});
     on_gpu(x);
     const int64_t threshold = (int64_t)std::nearbyint(p * 65536.0);
     if (wants_grad({x, residual})) return DropoutNode::apply(x, residual_, threshold, (int64_t)seed, (int64_t)offset, offset_t_);

@@ -8,7 +8,8 @@ The whole-sequence forms are differentiable in every floating-point input (the i
 are for acting.  Activations are float32, bfloat16 or float16, [B, T, D] with adjacent channels and any strides for batch and time (other layouts
 are copied); parameters, the scan's state and every sum are float32.  Everything runs on the current stream of the tensors' device, allocates
 from torch's caching allocator and reads nothing on the host, so calls can be captured in a hipGraph.  There is no CPU path.
-Arguments that do not fit raise ValueError, a failing launch RuntimeError; the gradients are not differentiable again.
+Arguments that do not fit raise ValueError, a failing launch RuntimeError; the gradients are not differentiable again, and a dual tensor
+(forward-mode derivatives) raises NotImplementedError.
 
 starts [B, T] (bool): step t is the first of a new sequence -- what came before, the incoming state included, does not reach it.
 lengths [B] (integers): row b has lengths[b] steps; outputs and gradients behind them are 0, inputs behind them are not looked at, and the
