@@ -5,8 +5,44 @@ evaluated over whole runs from a zero state, the state restarted behind `episode
 import torch
 
 
-def _kwargs(batch):
-    return dict(episode_dones=batch["episode_dones"], is_valid=batch.get("is_valid"))
+def _kwargs(batch, prefix=""):
+    return dict(episode_dones=batch[prefix + "episode_dones"], is_valid=batch.get(prefix + "is_valid"))
+
+
+def _check_runs(batch):
+    if batch["rewards"].ndim != 3:
+        raise ValueError(f"a recurrent agent is updated on [B, H, ...] batches (DeviceReplay with sampling_cfg=dict(type='TStepTransition', "
+                         f"horizon=...)); rewards are {tuple(batch['rewards'].shape)}")
+
+
+def with_target_history(batch):
+    """The batch with `next_obs` as the runs that the target's networks have to see.
+
+    What stands behind step t has the history obs[s], next_obs[s], ..., next_obs[t], with s the first step of t's episode in the run: the states
+    that the online networks reach one step later, and the policy when it acts.  Over next_obs alone the first observation of every episode
+    would be missing.  So each episode's first observation is put in front of its next ones: next_obs becomes [B, H + E, ...] (E: the most
+    episodes of a run), with next_episode_dones and next_is_valid to go with it, and next_at [B, H] says where next_obs[t] has gone."""
+    _check_runs(batch)
+    B, H = batch["rewards"].shape[:2]
+    ended = batch["episode_dones"].reshape(B, H).bool()
+    valid = torch.ones_like(ended) if batch.get("is_valid") is None else batch["is_valid"].reshape(B, H).bool()
+    starts = valid.clone()
+    starts[:, 1:] &= ended[:, :-1]
+    begun = starts.cumsum(1)                                   # episodes of the run up to and including step t's
+    episodes = int(begun[:, -1].max())
+    width, steps = H + episodes, torch.arange(H, device=ended.device).expand(B, H)
+    at = steps + begun
+    if episodes == 1:
+        pick = lambda first, rest: torch.cat((first[:, :1], rest), dim=1)
+    else:
+        # row numbers of (obs, next_obs) side by side; what is no start goes to a last place that is cut off
+        source = steps.new_zeros(B, width + 1).scatter_(1, at, H + steps).scatter_(1, torch.where(starts, at - 1, width), steps)[:, :width]
+        rows = torch.arange(B, device=ended.device)[:, None]
+        pick = lambda first, rest: torch.cat((first, rest), dim=1)[rows, source]
+    length = valid.sum(1, keepdim=True) + begun[:, -1:]
+    return dict(batch, next_obs={k: pick(batch["obs"][k], v) for k, v in batch["next_obs"].items()}, next_at=at[..., None],
+                next_episode_dones=torch.zeros(B, width, dtype=torch.bool, device=ended.device).scatter_(1, at, ended & valid)[..., None],
+                next_is_valid=(torch.arange(width, device=ended.device) < length)[..., None])
 
 
 def _mean(x, weight):
@@ -27,18 +63,19 @@ def _q_values(agent, critic, obs, actions, kw, feature=None):
 
 
 def recurrent_step(agent, batch, do_actor, polyak):
-    """One critic (and actor, temperature) step; returns the metrics of SAC._step_body."""
-    kw = _kwargs(batch)
-    rewards = batch["rewards"]
-    if rewards.ndim != 3:
-        raise ValueError(f"a recurrent agent is updated on [B, H, ...] batches (DeviceReplay with sampling_cfg=dict(type='TStepTransition', "
-                         f"horizon=...)); rewards are {tuple(rewards.shape)}")
+    """One critic (and actor, temperature) step; returns the metrics of SAC._step_body.  A batch without `next_at` (with_target_history) has
+    its target formed over next_obs as it stands."""
+    _check_runs(batch)
+    kw, rewards = _kwargs(batch), batch["rewards"]
+    at = batch.get("next_at")
+    next_kw = kw if at is None else _kwargs(batch, "next_")
     weight = torch.ones_like(rewards) if kw["is_valid"] is None else kw["is_valid"].to(rewards.dtype)
     stats = {}
     with torch.no_grad():
-        next_actions, neg_logp = agent.actor(batch["next_obs"], mode="max-entropy", save_feature=agent._dedup, **kw)
-        q_next = _q_values(agent, agent.target_critic, batch["next_obs"], next_actions, kw, agent.actor.backbone.pop_attr("saved_feature"))
+        next_actions, neg_logp = agent.actor(batch["next_obs"], mode="max-entropy", save_feature=agent._dedup, **next_kw)
+        q_next = _q_values(agent, agent.target_critic, batch["next_obs"], next_actions, next_kw, agent.actor.backbone.pop_attr("saved_feature"))
         min_q = q_next.min(dim=-1, keepdim=True).values + agent._alpha_t * neg_logp
+        min_q = min_q if at is None else min_q.gather(1, at)
         r = rewards * agent.reward_scale
         y = r + agent.gamma * min_q if agent.ignore_dones else r + (1 - batch["dones"].float()) * agent.gamma * min_q
     fb = agent._flat["critic"]

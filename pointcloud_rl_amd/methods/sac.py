@@ -576,8 +576,8 @@ class SAC(BaseAgent):
         if self._fused is not None:
             return self._fused.run(batch["obs"], batch["next_obs"], batch["actions"], batch["rewards"], batch["dones"], do_actor, polyak)
         if self.is_recurrent:
-            from .recurrent import recurrent_step
-            return recurrent_step(self, batch, do_actor, polyak)
+            from .recurrent import recurrent_step, with_target_history
+            return recurrent_step(self, with_target_history(batch), do_actor, polyak)
         stats = {}
         q_target = self._q_target(batch["next_obs"], batch["rewards"], batch["dones"])
         self._critic_step(batch["obs"], batch["actions"], q_target, stats, polyak=polyak)
