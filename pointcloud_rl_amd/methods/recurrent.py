@@ -15,6 +15,17 @@ def _check_runs(batch):
                          f"horizon=...)); rewards are {tuple(batch['rewards'].shape)}")
 
 
+def _blank(batch, padding):
+    """The batch with 0 in every floating-point tensor where padding [B, H] says so."""
+    def blank(v):
+        if isinstance(v, dict):
+            return {k: blank(x) for k, x in v.items()}
+        if not torch.is_tensor(v) or not v.is_floating_point() or v.shape[:2] != padding.shape:
+            return v
+        return v.masked_fill(padding.reshape(padding.shape + (1,) * (v.ndim - 2)), 0.0)
+    return {k: blank(v) for k, v in batch.items()}
+
+
 def with_target_history(batch):
     """The batch with `next_obs` as the runs that the target's networks have to see.
 
@@ -29,7 +40,9 @@ def with_target_history(batch):
     starts = valid.clone()
     starts[:, 1:] &= ended[:, :-1]
     begun = starts.cumsum(1)                                   # episodes of the run up to and including step t's
-    episodes = int(begun[:, -1].max())
+    episodes, whole = torch.stack((begun[:, -1].max(), valid.all().to(begun.dtype))).tolist()
+    if not whole:
+        batch = _blank(batch, ~valid)
     width, steps = H + episodes, torch.arange(H, device=ended.device).expand(B, H)
     at = steps + begun
     if episodes == 1:

@@ -142,6 +142,32 @@ def test_the_targets_features_are_the_online_ones_of_the_next_step(cuda):
     assert inside == 2 + 2 + 5 + 2
 
 
+@pytest.mark.gpu
+def test_padding_may_hold_anything(cuda):
+    """NaN and infinities behind the valid steps, in every tensor that can hold them: the metrics and gradients of clean padding."""
+    lengths, H = [5, 2, 4], 5
+    g = torch.Generator().manual_seed(9)
+    eps = [torch.randn(3, n, 4, generator=g).to(cuda) for n in (H + 1, H)]
+
+    def run(fill):
+        batch = make_batch(cuda, lengths, H)
+        for v in (batch["obs"]["xyz"], batch["next_obs"]["xyz"], batch["actions"], batch["rewards"]):
+            for b, n in enumerate(lengths):
+                v[b, n:] = fill
+        agent = make_agent(cuda)                         # (a step moves the temperature and the optimizers too)
+        agent.actor.head.noise_override = list(eps)
+        stats = agent._step_body(batch, True, False)
+        return {k: float(v) for k, v in stats.items()}, agent._flat["critic"].grad.clone(), agent._flat["actor"].grad.clone()
+
+    want = run(0.25)
+    assert all(np.isfinite(v) for v in want[0].values())
+    for fill in (float("nan"), float("inf")):
+        stats, critic, actor = run(fill)
+        assert stats == pytest.approx(want[0], rel=1e-5), fill
+        for a, b in ((critic, want[1]), (actor, want[2])):
+            assert float((a - b).norm() / b.norm()) < GRAD_TOL, fill
+
+
 def test_single_transitions_have_no_run():
     from pointcloud_rl_amd.methods.recurrent import with_target_history
     with pytest.raises(ValueError, match="TStepTransition"):
