@@ -17,7 +17,10 @@ class Dropout(ExtendedModule):
     """Counter-based dropout (sequence.dropout) with an optional residual, active in training mode.
 
     The seed is drawn from torch's generator when the module is made; the count of calls is the generator's offset and lives in device memory,
-    advanced by the call itself, so a captured step draws a new mask on every replay.  Neither is part of the state_dict."""
+    advanced by the call itself, so a captured step draws a new mask on every replay.  Neither is part of the state_dict.
+
+    A call inside a backward pass -- activation checkpointing, which evaluates a module a second time there -- is refused: it would draw the next
+    mask, not the one of the forward pass.  There, call sequence.dropout with an offset of your own."""
 
     def __init__(self, p):
         super().__init__()
@@ -30,6 +33,9 @@ class Dropout(ExtendedModule):
     def forward(self, x, residual=None):
         if not self.training or self.p == 0.0:
             return x if residual is None else x + residual
+        if torch._C._current_graph_task_id() != -1:
+            raise RuntimeError("Dropout is evaluated again inside a backward pass (activation checkpointing): its mask would not be the forward's; "
+                               "checkpoint a part without it, or call sequence.dropout with an offset of your own")
         self.calls.add_(1)
         return sequence.dropout(x, self.p, self.seed, self.calls.clone(), residual=residual)
 

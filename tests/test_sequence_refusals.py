@@ -31,3 +31,39 @@ def test_forward_mode_derivatives_are_refused(name, arg):
             getattr(sequence, name)(**dict(kw, **{arg: fwd.make_dual(kw[arg], torch.ones_like(kw[arg]))}))
         with pytest.raises(RuntimeError, match="no CPU path"):
             getattr(sequence, name)(**kw)
+
+
+def _checkpointed(x, module, reentrant):
+    from torch.utils.checkpoint import checkpoint
+    checkpoint(module, x, use_reentrant=reentrant).sum().backward()
+
+
+@pytest.mark.parametrize("reentrant", [False, True])
+def test_dropout_is_not_evaluated_again_in_a_backward_pass(monkeypatch, reentrant):
+    """Activation checkpointing would multiply the gradient with another mask than the forward's.  (The kernel is replaced: what is tested is
+    which calls reach it.)"""
+    from pointcloud_rl_amd.networks import Dropout, ssm
+    offsets = []
+    monkeypatch.setattr(ssm.sequence, "dropout", lambda x, p, seed, offset, residual=None: offsets.append(int(offset)) or x * x)
+    drop, x = Dropout(0.5), torch.ones(4, requires_grad=True)
+    with pytest.raises(RuntimeError, match="activation checkpointing"):
+        _checkpointed(x, drop, reentrant)
+    assert offsets == [1] and int(drop.calls) == 1
+    _checkpointed(x, drop.eval(), reentrant)             # nothing is drawn: fine
+    drop.train()(x).sum().backward()                     # an ordinary pass goes on
+    assert offsets == [1, 2]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("reentrant", [False, True])
+def test_dropout_under_activation_checkpointing(cuda, reentrant):
+    """The module refuses; the operator with an offset that the caller holds draws the forward's mask again."""
+    from pointcloud_rl_amd import sequence
+    from pointcloud_rl_amd.networks import Dropout
+    x = torch.randn(64, 33, device=cuda, requires_grad=True)
+    with pytest.raises(RuntimeError, match="activation checkpointing"):
+        _checkpointed(x, Dropout(0.5).to(cuda), reentrant)
+    x.grad = None
+    _checkpointed(x, lambda t: sequence.dropout(t, 0.5, 7, 3), reentrant)
+    want, = torch.autograd.grad(sequence.dropout(x, 0.5, 7, 3).sum(), x)
+    assert torch.equal(x.grad, want)
