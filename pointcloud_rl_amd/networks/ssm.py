@@ -17,7 +17,8 @@ class Dropout(ExtendedModule):
     """Counter-based dropout (sequence.dropout) with an optional residual, active in training mode.
 
     The seed is drawn from torch's generator when the module is made; the count of calls is the generator's offset and lives in device memory,
-    advanced by the call itself, so a captured step draws a new mask on every replay.  Neither is part of the state_dict.
+    advanced by the call itself, so a captured step draws a new mask on every replay.  Neither is part of the state_dict; checkpoints
+    (utils/checkpoint.py) keep both, so a resumed run draws the masks that the run would have drawn.
 
     A call inside a backward pass -- activation checkpointing, which evaluates a module a second time there -- is refused: it would draw the next
     mask, not the one of the forward pass.  There, call sequence.dropout with an offset of your own."""
@@ -38,6 +39,18 @@ class Dropout(ExtendedModule):
                                "checkpoint a part without it, or call sequence.dropout with an offset of your own")
         self.calls.add_(1)
         return sequence.dropout(x, self.p, self.seed, self.calls.clone(), residual=residual)
+
+    def checkpoint_state(self):
+        """What a checkpoint keeps beside the state_dict's entries."""
+        return dict(seed=torch.tensor([self.seed]), calls=self.calls.detach())
+
+    def _load_from_state_dict(self, state_dict, prefix, *args):
+        seed, calls = state_dict.pop(prefix + "seed", None), state_dict.pop(prefix + "calls", None)
+        if seed is not None and calls is not None:              # (a file without them leaves the module its own masks)
+            self.seed = int(seed)
+            with torch.no_grad():
+                self.calls.copy_(calls)
+        super()._load_from_state_dict(state_dict, prefix, *args)
 
     def extra_repr(self):
         return f"p={self.p}"

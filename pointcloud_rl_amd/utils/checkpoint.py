@@ -35,6 +35,9 @@ def get_state_dict(module, destination=None, prefix="", keep_vars=False):
     for name, buf in module._buffers.items():
         if buf is not None:
             destination[prefix + name] = buf if keep_vars else buf.detach()
+    if hasattr(module, "checkpoint_state"):        # a module with state that nn.Module.state_dict does not show (networks/ssm.py: Dropout)
+        for name, value in module.checkpoint_state().items():
+            destination[prefix + name] = value
     seen = set()
     for name, child in module.__dict__.items():
         if child is not None and _is_optimizer(child) and id(child) not in seen:
