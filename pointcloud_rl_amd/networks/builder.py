@@ -54,6 +54,9 @@ def build_target_network(network_cfg, network, shared_network=None, shared_backb
         target = build_all(_share_backbone_parts(network_cfg, shared_network))
     else:
         target = deepcopy(network)
+        for module in target.modules():
+            if hasattr(module, "reseed"):       # a copy draws masks of its own (networks/ssm.py: Dropout)
+                module.reseed()
     hard_update(target, network)
     disable_gradients(target, exclude=[id(p) for p in network.parameters()])
     return target

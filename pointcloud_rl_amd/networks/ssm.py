@@ -28,8 +28,12 @@ class Dropout(ExtendedModule):
         if not 0.0 <= float(p) < 1.0:
             raise ValueError(f"dropout probability {p}: 0 <= p < 1")
         self.p = float(p)
-        self.seed = int(torch.randint(0, 2 ** 62, (1,)).item())
+        self.reseed()
         self.register_buffer("calls", torch.zeros(1, dtype=torch.int64), persistent=False)
+
+    def reseed(self):
+        """Masks independent of every other module's from here on: a copied module otherwise draws its original's."""
+        self.seed = int(torch.randint(0, 2 ** 62, (1,)).item())
 
     def forward(self, x, residual=None):
         if not self.training or self.p == 0.0:

@@ -50,6 +50,17 @@ def test_files_without_masks_leave_a_module_its_own(tmp_path):
     assert (drop.seed, int(drop.calls)) == before
 
 
+@pytest.mark.parametrize("shared", [False, True])
+def test_online_and_target_networks_draw_masks_of_their_own(shared):
+    """The target network is built afresh or copied from the online one: no two of their Dropouts share a seed.  The weights are copies."""
+    agent = make_agent(0, shared_backbone=shared)
+    online, target = agent.critic, agent.target_critic
+    seeds = [d.seed for d in drops(online) + drops(target)]
+    assert len(seeds) == 8 and len(set(seeds)) == 8
+    for a, b in zip(online.parameters(), target.parameters()):
+        assert torch.equal(a, b)
+
+
 @pytest.mark.gpu
 def test_a_resumed_run_draws_the_masks_it_would_have_drawn(cuda, tmp_path):
     """Three steps, a checkpoint, three more in a freshly built agent: the parameters of six steps, to the bit."""
