@@ -42,7 +42,9 @@ class Dropout(ExtendedModule):
             raise RuntimeError("Dropout is evaluated again inside a backward pass (activation checkpointing): its mask would not be the forward's; "
                                "checkpoint a part without it, or call sequence.dropout with an offset of your own")
         self.calls.add_(1)
-        return sequence.dropout(x, self.p, self.seed, self.calls.clone(), residual=residual)
+        if residual is None or residual.dtype == x.dtype:
+            return sequence.dropout(x, self.p, self.seed, self.calls.clone(), residual=residual)
+        return residual + sequence.dropout(x, self.p, self.seed, self.calls.clone())         # the wider type, as without dropout
 
     def checkpoint_state(self):
         """What a checkpoint keeps beside the state_dict's entries."""
@@ -71,7 +73,10 @@ class SelectiveSSM(ExtendedModule):
 
     forward(x, states, starts, lengths) -> (y, states).  x [B, T, feat_dim]: a run of steps, differentiable in x and in the states it starts from;
     x [B, feat_dim]: one step (acting), without gradients and without dropout.  states: dict(conv [B, conv_width - 1, inner], ssm [B, inner,
-    state_dim]) or None (zeros); the returned ones follow the last step.  starts [B, T] / [B]: steps that begin a new episode; lengths [B]."""
+    state_dim]) or None (zeros); the returned ones follow the last step.  starts [B, T] / [B]: steps that begin a new episode; lengths [B].
+
+    The operators run in the type of the projections (float32, or 16 bits under autocast or with 16-bit weights: so does the convolution's state),
+    with their parameters and the scan's state in float32."""
 
     def __init__(self, feat_dim, expand=2, state_dim=16, conv_width=4, dt_rank="auto", groups=1, dropout=0.0, dt_range=(1e-3, 1e-1), **kwargs):
         super().__init__()
@@ -106,24 +111,27 @@ class SelectiveSSM(ExtendedModule):
         shape = v.shape[:-1] + (self.groups, self.state_dim)
         return F.linear(dt, self.dt_proj.weight), B.reshape(shape), C.reshape(shape)
 
+    def _scan_parameters(self):
+        return dict(A=-torch.exp(self.A_log.float()), D=self.D.float(), dt_bias=self.dt_proj.bias.float())
+
     def forward(self, x, states=None, starts=None, lengths=None):
         if x.ndim == 2:
             return self.step(x, states, starts)
         v, z = self.in_proj(self.norm(x)).chunk(2, dim=-1)
-        conv, ssm = (None, None) if states is None else (states["conv"], states["ssm"])
-        v, conv = sequence.short_conv(v, self.conv_weight, self.conv_bias, state=conv, starts=starts, lengths=lengths)
+        conv, ssm = (None, None) if states is None else (states["conv"].to(v.dtype), states["ssm"])
+        v, conv = sequence.short_conv(v, self.conv_weight.float(), self.conv_bias.float(), state=conv, starts=starts, lengths=lengths)
         dt, B, C = self._scan_inputs(v)
-        y, ssm = sequence.ssm_scan(v, dt, -torch.exp(self.A_log), B, C, D=self.D, z=z, dt_bias=self.dt_proj.bias, state=ssm, starts=starts, lengths=lengths)
+        y, ssm = sequence.ssm_scan(v, dt, B=B, C=C, z=z, state=ssm, starts=starts, lengths=lengths, **self._scan_parameters())
         y = self.out_proj(y)
         return (x + y if self.dropout is None else self.dropout(y, residual=x)), dict(conv=conv, ssm=ssm)
 
     @torch.no_grad()
     def step(self, x, states=None, starts=None):
         """One step for a batch of environments: x [B, feat_dim], starts [B] -> (y, new states); the given states are left as they are."""
-        states = self.init_states(x.shape[0], x.device, x.dtype) if states is None else states
-        conv, ssm = torch.empty_like(states["conv"]), torch.empty_like(states["ssm"])
         v, z = self.in_proj(self.norm(x)).chunk(2, dim=-1)
-        v = sequence.short_conv_step(v, states["conv"], self.conv_weight, self.conv_bias, starts=starts, state_out=conv)
+        states = self.init_states(x.shape[0], x.device, v.dtype) if states is None else dict(states, conv=states["conv"].to(v.dtype))
+        conv, ssm = torch.empty_like(states["conv"]), torch.empty_like(states["ssm"])
+        v = sequence.short_conv_step(v, states["conv"], self.conv_weight.float(), self.conv_bias.float(), starts=starts, state_out=conv)
         dt, B, C = self._scan_inputs(v)
-        y = sequence.ssm_step(v, dt, -torch.exp(self.A_log), B, C, states["ssm"], D=self.D, z=z, dt_bias=self.dt_proj.bias, starts=starts, state_out=ssm)
+        y = sequence.ssm_step(v, dt, B=B, C=C, state=states["ssm"], z=z, starts=starts, state_out=ssm, **self._scan_parameters())
         return x + self.out_proj(y), dict(conv=conv, ssm=ssm)
