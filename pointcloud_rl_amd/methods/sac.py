@@ -252,6 +252,9 @@ class SAC(BaseAgent):
         shared_target_backbone = shared_backbone if shared_target_backbone is None else shared_target_backbone
         self.target_critic = build_target_network(critic_cfg, self.critic, self.actor, shared_target_backbone)
         self.is_recurrent = bool(self.actor.is_recurrent)       # a recurrent core in the backbone (Visuomotor rnn_cfg)
+        if getattr(self.critic, "is_recurrent", False) and not self.is_recurrent:
+            raise ValueError("critic_cfg has a recurrent core (rnn_cfg) and actor_cfg has none: the agent would be updated on single transitions, "
+                             "which a core is not trained on")
 
         self.log_alpha = nn.Parameter(torch.ones(1, requires_grad=True))
         self.log_alpha.data *= float(np.log(np.float32(alpha)))

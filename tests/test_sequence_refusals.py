@@ -67,3 +67,16 @@ def test_dropout_under_activation_checkpointing(cuda, reentrant):
     _checkpointed(x, lambda t: sequence.dropout(t, 0.5, 7, 3), reentrant)
     want, = torch.autograd.grad(sequence.dropout(x, 0.5, 7, 3).sum(), x)
     assert torch.equal(x.grad, want)
+
+
+def test_a_recurrent_critic_without_a_recurrent_actor_is_refused():
+    """Such an agent counted as not recurrent: its step took the critic's core for absent."""
+    import copy
+    from pointcloud_rl_amd import configs
+    from pointcloud_rl_amd.methods import build_agent
+    cfg = configs.recurrent(configs.sac_dmc(6, 4, 6, head_hidden=64), state_dim=8)
+    cfg["env_params"] = configs.env_params({"xyz": [3, 64], "rgb": [3, 64]}, 4)
+    assert build_agent(copy.deepcopy(cfg)).is_recurrent
+    cfg["critic_cfg"]["nn_cfg"]["rnn_cfg"] = cfg["actor_cfg"]["nn_cfg"].pop("rnn_cfg")
+    with pytest.raises(ValueError, match="rnn_cfg"):
+        build_agent(cfg)
