@@ -616,7 +616,8 @@ typedef struct pcrl_conv_desc {
     const uint8_t* starts; int64_t starts_sb;
     const int32_t* lengths;
 } pcrl_conv_desc;
-/* y [B][T][D], last_state [B][W-1][D] (may be NULL).  last_state may be the memory of `state` only when T == 1 (the acting step). */
+/* y [B][T][D], last_state [B][W-1][D] (may be NULL).  last_state may be the memory of `state` only when T == 1 (the acting step), and may not
+ * touch it otherwise. */
 int pcrl_short_conv_fwd(const pcrl_conv_desc* d, void* y, void* last_state, void* stream);
 int pcrl_short_conv_bwd_workspace_bytes(const pcrl_conv_desc* d, size_t* bytes);
 /* Gradients of sum(y * dy) + sum(last_state * dlast): dx [B][T][D], dweight [D][W], dbias [D] or NULL, dstate [B][W-1][D] or NULL.
@@ -646,7 +647,7 @@ typedef struct pcrl_ssm_grads {
 /* workspace: what the forward needs (0 for most shapes); saved: what a forward that will be differentiated leaves for its backward (the state
  * in front of every 16th step); bwd: the backward's workspace. */
 int pcrl_ssm_scan_bytes(const pcrl_ssm_desc* d, size_t* workspace, size_t* saved, size_t* bwd);
-/* y [B][T][D], last_state [B][D][N] (may be NULL); saved NULL: no backward will follow. */
+/* y [B][T][D], last_state [B][D][N] (may be NULL; may not touch d->state); saved NULL: no backward will follow. */
 int pcrl_ssm_scan_fwd(const pcrl_ssm_desc* d, void* y, float* last_state, float* saved, void* workspace, size_t workspace_bytes, void* stream);
 /* Gradients of sum(y * dy) + sum(last_state * dlast) (dlast may be NULL), from the forward's inputs and `saved`.  No atomics: the same call
  * gives the same bits. */

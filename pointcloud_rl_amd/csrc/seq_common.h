@@ -133,6 +133,11 @@ __device__ __forceinline__ float dot_row_bcast(const float (&c)[RN], const float
 
 constexpr long long kMaxGroups = (1LL << 24) - 1;      // workgroups of 256: a grid holds fewer than 2^32 threads
 __host__ inline int elem_bytes(int dtype) { return dtype == PCRL_DT_F32 ? 4 : 2; }
+// Two ranges of memory touch each other without being the same one (same: also when they are).
+__host__ inline bool overlap(const void* a, const void* b, size_t bytes, bool same) {
+    const uintptr_t x = (uintptr_t)a, y = (uintptr_t)b;
+    return a && b && (x != y ? (x < y ? y - x : x - y) < bytes : same);
+}
 __host__ inline bool seq_dtype(int dtype) { return dtype == PCRL_DT_F32 || dtype == PCRL_DT_BF16 || dtype == PCRL_DT_F16; }
 
 }  // namespace pcrl

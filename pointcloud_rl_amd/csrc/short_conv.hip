@@ -446,7 +446,8 @@ using namespace pcrl;
 extern "C" int pcrl_short_conv_fwd(const pcrl_conv_desc* d, void* y, void* last_state, void* stream) {
     if (int rc = conv_check(d, "pcrl_short_conv_fwd")) return rc;
     if (!y) return fail(PCRL_E_ARG, "pcrl_short_conv_fwd: null output");
-    if (d->T > 1 && last_state && last_state == d->state) return fail(PCRL_E_ARG, "pcrl_short_conv_fwd: the state is updated in place by a single step only (T = %d)", d->T);
+    if (overlap(last_state, d->state, (size_t)d->B * (d->W - 1) * d->D * elem_bytes(d->dtype), d->T > 1))
+        return fail(PCRL_E_ARG, "pcrl_short_conv_fwd: last_state overlaps state (T = %d; a single step may update it in place)", d->T);
     ConvParams p;
     conv_fill(p, d);
     p.y = y, p.last = last_state;

@@ -389,6 +389,8 @@ extern "C" int pcrl_ssm_scan_bytes(const pcrl_ssm_desc* d, size_t* workspace, si
 extern "C" int pcrl_ssm_scan_fwd(const pcrl_ssm_desc* d, void* y, float* last_state, float* saved, void* workspace, size_t workspace_bytes, void* stream) {
     if (int rc = ssm_check(d, "pcrl_ssm_scan_fwd")) return rc;
     if (!y) return fail(PCRL_E_ARG, "pcrl_ssm_scan_fwd: null output");
+    // (every chunk reads the state, the last one writes last_state)
+    if (overlap(last_state, d->state, sizeof(float) * d->B * d->D * d->N, true)) return fail(PCRL_E_ARG, "pcrl_ssm_scan_fwd: last_state overlaps state");
     const SsmPlan plan = ssm_plan(d, false);
     const size_t need = fwd_workspace(d, plan);
     if (need && (!workspace || workspace_bytes < need)) return fail(PCRL_E_WORKSPACE, "pcrl_ssm_scan_fwd: workspace %zu < %zu", workspace_bytes, need);
@@ -411,6 +413,7 @@ extern "C" int pcrl_ssm_step(const pcrl_ssm_desc* d, void* y, float* state_out, 
     if (int rc = ssm_check(d, "pcrl_ssm_step")) return rc;
     if (d->T != 1) return fail(PCRL_E_ARG, "pcrl_ssm_step: T = %d", d->T);
     if (!y || !state_out || !d->state) return fail(PCRL_E_ARG, "pcrl_ssm_step: null output or state");
+    if (overlap(state_out, d->state, sizeof(float) * d->B * d->D * d->N, false)) return fail(PCRL_E_ARG, "pcrl_ssm_step: state_out overlaps the state without being it");
     SsmStepParams q;
     ssm_fill(q.s, d);
     q.s.y = y, q.state_out = state_out;

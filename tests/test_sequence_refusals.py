@@ -80,3 +80,30 @@ def test_a_recurrent_critic_without_a_recurrent_actor_is_refused():
     cfg["critic_cfg"]["nn_cfg"]["rnn_cfg"] = cfg["actor_cfg"]["nn_cfg"].pop("rnn_cfg")
     with pytest.raises(ValueError, match="rnn_cfg"):
         build_agent(cfg)
+
+
+def test_states_that_overlap_are_refused_at_the_c_entry_points():
+    """A last state in the memory of the incoming one: chunks of the scan and runs of the convolution would read what others have written.  Nothing
+    is dereferenced: the calls that are not refused here fail on a later check (no scratch, a null output)."""
+    import ctypes
+    from pointcloud_rl_amd import _lib
+    from test_sequence_gpu import ConvDesc, SsmDesc
+    lib = _lib.lib()
+    at = lambda v: ctypes.c_void_p(v)
+    y, none, base = at(1 << 40), ctypes.c_size_t(0), 1 << 20
+
+    def scan(last, T=64):
+        d = SsmDesc(B=2, T=T, D=8, N=4, G=1, u=4096, dt=4096, Bm=4096, Cm=4096, A=4096, state=base)
+        return lib.pcrl_ssm_scan_fwd(ctypes.byref(d), y, at(last), None, None, none, None)
+
+    size = 4 * 2 * 8 * 4
+    for last in (base, base + 4, base - 4, base + size - 4, base - size + 4):
+        assert scan(last) == -1 and b"overlaps" in lib.pcrl_last_error(), last
+    for last in (base + size, base - size):
+        assert scan(last) == -2 and b"workspace" in lib.pcrl_last_error(), last      # 64 steps of one block: chunks, which need scratch
+    for T, last in ((2, base), (2, base + 4), (1, base + 4), (1, base - 2 * 3 * 8 * 4 + 4)):
+        d = ConvDesc(B=2, T=T, D=8, W=4, x=4096, weight=4096, state=base)
+        assert lib.pcrl_short_conv_fwd(ctypes.byref(d), y, at(last), None) == -1 and b"overlaps" in lib.pcrl_last_error(), (T, last)
+    for out in (base + 4, base - size + 4):
+        d = SsmDesc(B=2, T=1, D=8, N=4, G=1, u=4096, dt=4096, Bm=4096, Cm=4096, A=4096, state=base)
+        assert lib.pcrl_ssm_step(ctypes.byref(d), y, at(out), None) == -1 and b"overlaps" in lib.pcrl_last_error(), out
