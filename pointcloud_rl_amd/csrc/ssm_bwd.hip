@@ -9,7 +9,8 @@
 // as soon as both exist (each lane keeps one and sends the other: 3 instructions for 2 values instead of 6 for each value's own tree), left per
 // channel block, and added up in a fixed order by a second launch.
 // Bound by vector instructions (at 16.8 M elements, N = 16: 96 M of a wave's, 23 a state and step, 187 us of every SIMD at 4.3 cycles each; the
-// 235 MB it cannot do without would take 44 us) at two waves per SIMD: 256 registers, the states and decays of a tile 128 of them.
+// 235 MB it cannot do without would take 44 us) at two waves per SIMD: 256 registers, the states and decays of a tile 128 of them.  More than 8 states
+// do not fit them: 8 registers spill in 16 bits and 19 in float32 (26 and 41 where accesses are single elements), 88 to 129 with two state groups.
 // Measured at 4 x 2048 x 2048, bf16: 80 us for the chunk summaries, 257 us for the walk, 10 us for the sums.  What was slower for the walk: LDS
 // reads one group of steps ahead (302, it spills), states of half a tile at a time (264), the next tile's loads in the middle of the walk (275).
 #include "ssm_common.h"

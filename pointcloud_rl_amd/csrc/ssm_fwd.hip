@@ -288,6 +288,9 @@ int ssm_check(const pcrl_ssm_desc* d, const char* who) {
     return PCRL_OK;
 }
 
+// One answer for all of them: where B and C admit no whole vectors, the activations are read element by element too.  392 channels, N = 16, B and C
+// slices from element 13 of rows of 45, float32, in a graph, us (dense / slices): training pass of 256 x 16 63 / 88, of 4 x 1024 94 / 215; the step's
+// own rule below is of the same kind: 1024 rows 17 / 27.
 bool ssm_vec(const pcrl_ssm_desc* d, const void* const* extra, const long long* strides, int n_extra) {
     const size_t bytes = 4 * (size_t)elem_bytes(d->dtype);
     if ((d->D / d->G) % 4) return false;
@@ -325,6 +328,8 @@ void ssm_fill(SsmParams& p, const pcrl_ssm_desc* d) {
 // chunks: 128 blocks 321 / 818, 262 / 492, 174 / 343, 152 / 335; 256 blocks 162 / 376, 154 / 329, 140 / 327, -; 384 blocks (25 M elements) 189 / 496,
 // 208 / 498, 208 / 482, -; 512 blocks 104 / 268, 126 / 307, 139 / 333, -.  So: none from 1.5 blocks per CU on, else up to 4 workgroups per CU forward
 // and 2 backward (its registers and LDS admit no more), down to single tiles (333 steps, 28 blocks: 21 chunks 19 / 33, 11 chunks 21 / 37, 7 chunks 21 / 38).
+// Every chunk reads the summaries of all chunks in front of it, and nothing bounds their number: one block of a long sequence pays for that (64
+// channels, forward / training pass in a graph, us: 2048 steps 41 / 83, 4096 70 / 143, 8192 -- 512 chunks -- 167 / 323).
 SsmPlan ssm_plan(const pcrl_ssm_desc* d, bool backward) {
     SsmPlan plan{};
     const int ntile = cdiv(d->T, kTile);
