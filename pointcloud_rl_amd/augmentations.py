@@ -63,7 +63,7 @@ def _as_augmented(data):
 
 def _batch_shape(data):
     """Shape of the xyz tensor the augmentation acts on: [rows of the (virtually repeated) batch, 3, N]."""
-    return (batch_rows(data),) + tuple(data["xyz"].shape[1:])
+    return (batch_rows(data),) + tuple(data["xyz"].shape[-2:])
 
 
 class _PointAug:
@@ -152,7 +152,7 @@ class RandomDownSample:
 
     def __call__(self, data):
         assert self.main_key in data, f"{self.main_key}, {list(data.keys())}"
-        point_keys = [k for k, v in data.items() if torch.is_tensor(v) and v.ndim == 3]
+        point_keys = [k for k, v in data.items() if torch.is_tensor(v) and v.ndim == data[self.main_key].ndim]
         missing = [k for k in point_keys if k not in self.req_keys]
         if missing:
             raise NotImplementedError(f"RandomDownSample: point-cloud keys {missing} are not in req_keys {self.req_keys}; "
@@ -244,7 +244,7 @@ class ColorJitterPoints:
                                       f"(torchvision's float path differs), got {rgb.dtype}")
         order, factors = self.draw()
         color = dict(order=order, factors=factors)
-        color["mean"] = hip.color_contrast_mean(rgb, color)      # [stored clouds]: a virtual repeat shares it
+        color["mean"] = hip.color_contrast_mean(rgb.reshape((-1,) + tuple(rgb.shape[-2:])), color)      # [stored clouds]: a virtual repeat shares it
         out = _as_augmented(data)
         out.aug["color"] = color
         return out

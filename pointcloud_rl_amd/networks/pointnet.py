@@ -6,6 +6,7 @@ pyrl/networks/backbones/pointnet.py:76-157; parameter names follow its state_dic
 The per-point MLP, its LayerNorms, the max-pool and their backward run in libpcrl_hip.so; there
 is no eager or CPU path.
 """
+import math
 import os
 
 import torch
@@ -31,8 +32,25 @@ class AugmentedObs(dict):
 
 
 def batch_rows(obs):
-    """Rows of the batch an observation dict stands for (stored rows x repeat)."""
-    return obs["xyz"].shape[0] * int(getattr(obs, "repeat", 1) or 1)
+    """Rows of the batch an observation dict stands for (stored rows x repeat); every cloud of a run of steps [B, T, C, N] is a row."""
+    return math.prod(obs["xyz"].shape[:-2]) * int(getattr(obs, "repeat", 1) or 1)
+
+
+def checked_aug_desc(aug, desc):
+    """The augmentation's descriptor for the clouds of `desc` (None without one).  The kernels read one row of its per-cloud tensors for every
+    cloud, row b * row_mul + row_add: tensors that do not reach that far are refused here."""
+    if not aug:
+        return None
+    rows = max(desc.B - 1, 0) * (int(aug.get("row_mul", 1)) or 1) + int(aug.get("row_add", 0)) + 1
+    index = aug.get("point_index")
+    n = desc.N if index is None else index.numel()
+    color = aug.get("color") or {}
+    for name, t, need in (("affine", aug.get("affine"), rows * 12), ("jitter_noise", aug.get("jitter_noise"), rows * 3 * n),
+                          ("color mean", color.get("mean"), -(-desc.B // max(desc.row_div, 1)))):
+        if t is not None and (t.numel() < need or not t.is_contiguous() or t.dtype != torch.float32 or not t.is_cuda):
+            raise ValueError(f"{name} of an augmentation is {t.dtype} {tuple(t.shape)} on {t.device}: {desc.B} clouds of {desc.N} points read {need} "
+                             "contiguous float32 values on the device")
+    return hip.make_aug_desc(**aug)
 
 
 def materialize(obs):
@@ -84,7 +102,7 @@ class _EncoderFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, net, desc, keep, aug, *weights):
         ew, packed = net._weights_desc()
-        aug_desc = hip.make_aug_desc(**aug) if aug else None
+        aug_desc = checked_aug_desc(aug, desc)
         pooled, argmax = hip.encoder_fwd(desc, ew, packed, aug=aug_desc, workspace=net._workspace("fwd"), bf16=net.compute_dtype == "bf16",
                                          split=net.compute_dtype == "f32split")
         ctx.net, ctx.desc, ctx.keep, ctx.aug_desc, ctx.aug = net, desc, keep, aug_desc, aug
@@ -210,7 +228,7 @@ class PointNet(ExtendedModule):
             inputs = {"xyz": inputs.to(dtype=torch.float32)}
         desc, keep = hip.make_cloud_desc(inputs)
         ew, packed = self._weights_desc()
-        aug_desc = hip.make_aug_desc(**aug) if aug else None
+        aug_desc = checked_aug_desc(aug, desc)
         pooled, argmax = hip.encoder_fwd(desc, ew, packed, aug=aug_desc, workspace=self._workspace("fwd"), bf16=self.compute_dtype == "bf16",
                                          split=self.compute_dtype == "f32split", head=head)
         return pooled, argmax, (desc, keep, aug, aug_desc, ew, packed, pooled)
@@ -221,7 +239,7 @@ class PointNet(ExtendedModule):
         aug = getattr(inputs, "aug", None)
         desc, keep = hip.make_cloud_desc(inputs)
         ew, packed = self._weights_desc()
-        return desc, keep, aug, (hip.make_aug_desc(**aug) if aug else None), ew, packed, pooled
+        return desc, keep, aug, checked_aug_desc(aug, desc), ew, packed, pooled
 
     def can_prepare(self, ctx):
         """Whether backward_prepare would launch (exact fp32 arithmetic, the forward's pooled values at hand, at most 2 048 clouds)."""

@@ -64,6 +64,8 @@ class Visuomotor(ExtendedModule):
             return visual_feature
         steps = None
         if self.rnn is not None and isinstance(visual, dict) and any(v.ndim == 4 for v in visual.values()):
+            if getattr(visual, "repeat", 1) not in (None, 1):
+                raise NotImplementedError("a run of steps is not encoded several times over (a virtually repeated observation)")
             steps = next(iter(visual.values())).shape[:2]          # a run of steps: every cloud of it is one row of the encoder's batch
             flat = copy(visual)
             for k in list(flat.keys()):

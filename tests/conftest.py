@@ -27,7 +27,7 @@ def cuda():
 _GPU_FILE_ORDER = [
     "test_encoder_fwd_gpu.py", "test_encoder_bwd_gpu.py", "test_dense_tail_gpu.py", "test_gemm_plan.py", "test_headtail_gpu.py",
     "test_update_step_gpu.py", "test_fullsize_parity_gpu.py", "test_k2_fullsize_bf16_gpu.py",
-    "test_sequence_gpu.py", "test_sequence_plans.py", "test_sequence_views.py", "test_sequence_refusals.py", "test_recurrent_gpu.py", "test_recurrent_update.py", "test_recurrent_types.py", "test_dropout_streams.py", "test_aux_aug_acting_gpu.py", "test_color_jitter_gpu.py", "test_cabi_exports.py", "test_integration_stub_gpu.py",
+    "test_sequence_gpu.py", "test_sequence_plans.py", "test_sequence_views.py", "test_sequence_refusals.py", "test_recurrent_gpu.py", "test_recurrent_update.py", "test_recurrent_types.py", "test_run_augmentations.py", "test_dropout_streams.py", "test_aux_aug_acting_gpu.py", "test_color_jitter_gpu.py", "test_cabi_exports.py", "test_integration_stub_gpu.py",
     "test_reference_integration.py", "test_data_parallel_gpu.py",
 ]
 _LAST_TESTS = ("test_bench_dry_run_of_the_eight_rank_launch",)
