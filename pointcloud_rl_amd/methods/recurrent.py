@@ -34,6 +34,8 @@ def with_target_history(batch):
     would be missing.  So each episode's first observation is put in front of its next ones: next_obs becomes [B, H + E, ...] (E: the most
     episodes of a run), with next_episode_dones and next_is_valid to go with it, and next_at [B, H] says where next_obs[t] has gone."""
     _check_runs(batch)
+    if any(getattr(batch[k], "aug", None) or getattr(batch[k], "repeat", 1) not in (None, 1) for k in ("obs", "next_obs")):
+        raise ValueError("observations are augmented behind with_target_history: its rows are not the ones that the draws were made for")
     B, H = batch["rewards"].shape[:2]
     ended = batch["episode_dones"].reshape(B, H).bool()
     valid = torch.ones_like(ended) if batch.get("is_valid") is None else batch["is_valid"].reshape(B, H).bool()

@@ -580,7 +580,7 @@ class SAC(BaseAgent):
             return self._fused.run(batch["obs"], batch["next_obs"], batch["actions"], batch["rewards"], batch["dones"], do_actor, polyak)
         if self.is_recurrent:
             from .recurrent import recurrent_step, with_target_history
-            return recurrent_step(self, with_target_history(batch), do_actor, polyak)
+            return recurrent_step(self, batch if "next_at" in batch else with_target_history(batch), do_actor, polyak)
         stats = {}
         q_target = self._q_target(batch["next_obs"], batch["rewards"], batch["dones"])
         self._critic_step(batch["obs"], batch["actions"], q_target, stats, polyak=polyak)
@@ -879,6 +879,9 @@ class SAC(BaseAgent):
         def fetch(launch=True):
             sample = memory.sample(self.batch_size) if launch else memory.sample(self.batch_size, launch=False)
             sampled_batch = sample.to_torch(device=self.device, non_blocking=True)
+            if self.is_recurrent:                      # in front of the pre-processor: it draws for the rows that will be encoded
+                from .recurrent import with_target_history
+                sampled_batch = with_target_history(sampled_batch)
             if self._process_sampled_obs:          # sac.py:106 (drq.py's update_parameters does not call it)
                 sampled_batch = self.process_obs(sampled_batch)
             if self.use_episode_dones:

@@ -168,6 +168,57 @@ def test_padding_may_hold_anything(cuda):
             assert float((a - b).norm() / b.norm()) < GRAD_TOL, fill
 
 
+class _Flat:
+    """A pre-processor that leaves a pending augmentation: every cloud's coordinates times 0."""
+
+    def __init__(self):
+        self.shapes = []
+
+    def __call__(self, data):
+        from pointcloud_rl_amd.networks.pointnet import AugmentedObs, batch_rows
+        out = AugmentedObs(data["obs"])
+        out.aug = dict(affine=torch.zeros(batch_rows(out), 3, 4, device=out["xyz"].device))
+        self.shapes.append(tuple(out["xyz"].shape))
+        return dict(data, obs=out)
+
+
+@pytest.mark.gpu
+def test_a_pre_processors_augmentation_reaches_the_encoder(cuda):
+    """Its draws are made for the target's rows too, and what it leaves pending is applied: with every coordinate taken to 0 the update does not
+    depend on the coordinates."""
+    from pointcloud_rl_amd.replay import DeviceReplay
+
+    def update(scale, flat):
+        agent = make_agent(cuda)
+        if flat is not None:
+            from pointcloud_rl_amd.augmentations import build_data_augmentations
+            agent.obs_processor = build_data_augmentations([flat])
+        mem = DeviceReplay(64, device=cuda, sampling_cfg=dict(type="TStepTransition", horizon=4, seed=5))
+        g = np.random.RandomState(5)
+        obs = lambda: {"xyz": (scale * g.randn(20, 3, 64)).astype(np.float32), "rgb": g.randint(0, 256, (20, 3, 64)).astype(np.uint8)}
+        mem.push_batch(dict(obs=obs(), next_obs=obs(), actions=g.uniform(-1, 1, (20, 4)).astype(np.float32), rewards=g.randn(20, 1).astype(np.float32),
+                            dones=np.zeros((20, 1), bool), episode_dones=np.zeros((20, 1), bool)))
+        noise = torch.Generator().manual_seed(9)
+        agent.actor.head.noise_override = [torch.randn(3, 5, 4, generator=noise).to(cuda)]
+        return agent.update_parameters(mem, 1)["sac/critic_loss"]
+
+    flat = _Flat()
+    assert update(1.0, flat) == update(2.0, flat)
+    assert update(1.0, None) != update(2.0, None)
+    assert flat.shapes == [(3, 4, 3, 64), (3, 5, 3, 64)] * 2
+
+
+def test_observations_are_augmented_behind_the_history():
+    from pointcloud_rl_amd.methods.recurrent import with_target_history
+    from pointcloud_rl_amd.networks.pointnet import AugmentedObs
+    batch = make_batch("cpu", [3, 2], 3)
+    batch["next_obs"] = AugmentedObs(batch["next_obs"])
+    with_target_history(batch)                           # nothing pending
+    batch["next_obs"].aug = dict(affine=torch.zeros(6, 3, 4))
+    with pytest.raises(ValueError, match="augmented"):
+        with_target_history(batch)
+
+
 def test_single_transitions_have_no_run():
     from pointcloud_rl_amd.methods.recurrent import with_target_history
     with pytest.raises(ValueError, match="TStepTransition"):
